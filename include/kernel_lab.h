@@ -104,6 +104,25 @@ int kl_rms_norm_grouped(kl_dtype dtype, void* out, const void* x, const void* re
                         int64_t x_group_stride, int64_t x_row_stride, float eps, kl_stream_t stream);
 
 /*
+ * kl_rms_norm_grouped with an output in OCP FP8 E4M3 ("e4m3fn") and fp32 scales,
+ * as an 8-bit projection takes its input. No counterpart in the reference.
+ *
+ *   y      = rmsnorm(x) * weight, or of the new residual; fp32, not rounded to
+ *            the input's type first
+ *   scales = max(max |y| / 448, 2^-126) over the finite y of a scale group:
+ *            scale_group consecutive columns (32, 64, 128 or 256, dividing
+ *            hidden), or the row (scale_group 0 or hidden)
+ *   out    = e4m3(y / scale), round to nearest even; a y that is not finite
+ *            becomes a NaN code
+ *
+ * `out` is [rows, hidden] bytes, `scales` [rows, hidden / scale_group] fp32, both
+ * contiguous; the other arguments are those of kl_rms_norm_grouped.
+ */
+int kl_rms_norm_fp8(kl_dtype dtype, void* out, float* scales, const void* x, const void* residual, void* residual_out,
+                    const void* weight, int64_t groups, int64_t rows_per_group, int64_t hidden,
+                    int64_t x_group_stride, int64_t x_row_stride, int64_t scale_group, float eps, kl_stream_t stream);
+
+/*
  * Split planning for paged decode. Pure host arithmetic: it reads no device
  * memory (in particular not seq_lens), so it never synchronises.
  * Follows choose_num_splits and the split normalisation of
@@ -252,6 +271,92 @@ int kl_paged_decode_attention_fp8(kl_dtype dtype, void* out, const void* q,
                                   int page_size, int64_t block_table_stride, int max_pages,
                                   float scale, int num_splits, void* workspace,
                                   size_t workspace_bytes, kl_stream_t stream);
+
+/*
+ * kl_paged_decode_attention_fp8 with a scale per page and KV head: k_scale and
+ * v_scale are [num_pages, num_kv_heads] fp32, and page p's codes of head h stand
+ * for k_scale[p, h] * decode(k) and v_scale[p, h] * decode(v). A scale is known
+ * when its page is written (kl_append_kv_fp8), and a large token costs its own
+ * page its precision, not the whole cache. No counterpart in the reference.
+ *
+ * head_tables 0: block_table [batch, stride] and seq_lens [batch], as above.
+ * head_tables 1: every (sequence, KV head) has a table and a length of its own,
+ * block_table [batch, num_kv_heads, stride] and seq_lens [batch, num_kv_heads],
+ * as kl_select_pages writes them; size the workspace with kl_paged_decode_plan
+ * for batch * num_kv_heads sequences of num_q_heads / num_kv_heads query heads and
+ * one KV head. Other arguments, refusals and results as
+ * kl_paged_decode_attention_fp8; a length of 0 gives zeros.
+ */
+int kl_paged_decode_attention_fp8_pages(kl_dtype dtype, void* out, const void* q, const void* k_cache,
+                                        const void* v_cache, const float* k_scale, const float* v_scale,
+                                        const int32_t* block_table, const int32_t* seq_lens, int batch,
+                                        int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                        int64_t block_table_stride, int max_pages, int head_tables, float scale,
+                                        int num_splits, void* workspace, size_t workspace_bytes, kl_stream_t stream);
+
+/*
+ * Writes new tokens into a paged FP8 cache with a scale per page and KV head, in
+ * place. No counterpart in the reference, whose tests fill their caches.
+ *
+ *   k, v         [tokens, num_kv_heads, head_dim] of `dtype` (fp32, fp16, bf16);
+ *                token and head strides in elements, the head_dim contiguous
+ *   new_offsets  [batch + 1] int32: rows new_offsets[b] .. new_offsets[b + 1] - 1
+ *                are sequence b's; null: one row per sequence, tokens == batch
+ *   seq_lens     [batch] int32, the lengths with the new tokens: they take the
+ *                last positions
+ *   k_bounds     [num_pages, num_kv_heads, 2, head_dim] e4m3 or null: the smallest
+ *                and the largest code of the page's keys in each dimension
+ *                (kl_select_pages reads them)
+ *
+ * On each page, for k and v and each head: with new = max(max |x| / 448, 2^-126)
+ * over the finite new values, a page on which no earlier token of the sequence lies takes the scale
+ * new; one that holds earlier tokens takes max(old scale, new), and where that is
+ * larger its codes c become e4m3((decode(c) * old) / scale). The new codes are
+ * e4m3(x / scale), rounded to nearest even; a value that is not finite becomes a
+ * NaN code, which no bound takes in. Slots behind the last token are not written.
+ *
+ * Left alone, and nothing of theirs written: sequences whose length is less than
+ * their new tokens (a padded batch gives them length 0) and whose offsets are not
+ * within the rows; the tokens of a page whose column is not below max_pages or whose
+ * id is not in [0, num_pages). Two
+ * sequences must not append to the same page in one call. Asynchronous on
+ * `stream`, no workspace.
+ */
+int kl_append_kv_fp8(kl_dtype dtype, void* k_cache, void* v_cache, float* k_scale, float* v_scale, void* k_bounds,
+                     const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, const int32_t* block_table,
+                     const int32_t* seq_lens, const int32_t* new_offsets, int64_t tokens, int batch,
+                     int num_kv_heads, int head_dim, int page_size, int num_pages, int64_t block_table_stride,
+                     int max_pages, kl_stream_t stream);
+
+/*
+ * Chooses the pages that each (sequence, KV head) attends, by a bound on their
+ * keys: sparse decode is kl_select_pages, then kl_paged_decode_attention_fp8_pages
+ * over the tables it writes. No counterpart in the reference.
+ *
+ *   score = f32(k_scale * max over the KV head's query heads of
+ *               sum_d max(q_d * lo_d, q_d * hi_d))
+ * with lo and hi the decoded codes of k_bounds: no key of the page has a larger
+ * q.k. The sums are formed in 64 bits. A NaN score counts as the largest finite one.
+ * The first `first_pages` pages of a sequence and its last `last_pages` come
+ * before all others; of the rest the largest scores are kept, equal ones lowest
+ * page first, num_selected pages in all, or every page of a shorter sequence.
+ *
+ *   out_table  [batch, num_kv_heads, num_selected] int32: the kept pages' ids from
+ *              block_table in the order of the sequence, padded with 0
+ *   out_lens   [batch, num_kv_heads] int32: the tokens on them
+ *   workspace  at least kl_select_pages_workspace's bytes (host arithmetic)
+ *
+ * q [batch, num_q_heads, head_dim] fp16 or bf16; head_dim 64, 128 or 256; first_pages
+ * >= 0, last_pages >= 1, first_pages + last_pages <= num_selected.
+ */
+int kl_select_pages_workspace(int batch, int num_kv_heads, int max_pages, size_t* out_workspace);
+
+int kl_select_pages(kl_dtype dtype, int32_t* out_table, int32_t* out_lens, const void* q, const void* k_bounds,
+                    const float* k_scale, const int32_t* block_table, const int32_t* seq_lens, int batch,
+                    int num_q_heads, int num_kv_heads, int head_dim, int page_size, int64_t block_table_stride,
+                    int max_pages, int num_selected, int first_pages, int last_pages, void* workspace,
+                    size_t workspace_bytes, kl_stream_t stream);
 
 /*
  * Cascade (shared-prefix) decode: sequence b attends over the prefix_len[0]

@@ -37,7 +37,7 @@ CSRC = HERE / "csrc"
 PKG = HERE / "kernel_lab"
 INCLUDE = HERE.parent / "include"
 
-HIP_SOURCES = ["rmsnorm.hip", "paged_decode.hip"]
+HIP_SOURCES = ["rmsnorm.hip", "rmsnorm_fp8.hip", "paged_decode.hip", "fp8_cache.hip"]
 HOST_SOURCES = ["status.cpp"]
 
 # Packed-FP32 VALU forms are disabled on purpose: scalar and float2 code must

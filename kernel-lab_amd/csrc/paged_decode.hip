@@ -175,6 +175,11 @@ struct DecodeArgs {
   uint32_t table_magic;
   int table_shift;
   int table_tokens;
+  // PageScaled caches: KV heads of the cache (k_scale and v_scale are [num_pages,
+  // cache_heads]), and how many of them have block tables of their own: 0, or all,
+  // where `batch` counts (sequence, KV head) pairs and num_kv_heads is 1.
+  int cache_heads;
+  int list_heads;
 };
 
 // seq_lens as the kernels count it: at most what max_pages pages hold.
@@ -206,6 +211,17 @@ template <typename KVF>
 constexpr bool kSmallPages = false;
 template <typename F>
 constexpr bool kSmallPages<SmallPages<F>> = true;
+
+// FP8 codes with a scale per page and KV head instead of one per KV head. A
+// block lies within a page, so its scales are two wave-uniform numbers, which
+// travel with its K and V loads: the scores take k_scale in place of the head's
+// scale, and v_scale goes into the softmax weights ahead of the P V product (the
+// normaliser takes the weights without it). The product of a weight and a scale
+// can be any fp32 value, so P and V are bf16 whatever the queries are (every code
+// is exact in bf16, and P's pair keeps 2^-17 of a weight).
+struct PageScaled : Fp8E4M3 {};
+template <typename KVF>
+constexpr bool kPageScaled = std::is_base_of_v<PageScaled, KVF>;
 
 // Whether the softmax weights keep fp32's precision up to the P V products, as
 // the VALU kernel's do: fp32, and small pages, which are 16-bit caches whose
@@ -556,6 +572,8 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
   constexpr bool KV8 = KVF::kBytes == 1;
   constexpr bool FP32 = std::is_same_v<E, F32>;
   constexpr bool SP = kSmallPages<KVF>;
+  constexpr bool PS = kPageScaled<KVF>;
+  using PE = std::conditional_t<PS, BF16, E>;  // the type of P and V in their product
   constexpr bool P32 = fp32_weights<E, KVF>();
   // log2 of the weight that moves the reference max, and of the weight the
   // score that moved it then has. P32: bf16 weights stay at most 1, so that a
@@ -617,10 +635,13 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
   // Score scale (log2 domain) and output scale of this KV head.
   float qk_scale = a.scale_log2;
   float out_scale = 1.0f;
-  if constexpr (KV8) {
+  if constexpr (KV8 && !PS) {
     qk_scale *= as_constant(a.k_scale)[u.kvh];
     out_scale = as_constant(a.v_scale)[u.kvh];
   }
+  // The cache's KV head, which a unit of a PageScaled cache with block tables per
+  // KV head has in u.b.
+  const int cache_head = PS && a.list_heads != 0 ? u.b % a.list_heads : u.kvh;
   const const_i32_ptr bt = as_constant(a.block_table + static_cast<int64_t>(u.b) * a.bt_stride);
   const int bpp = a.page_size / kBlock;  // blocks per page
   const int blk_begin = SP ? 0 : u.page_begin * bpp;
@@ -707,7 +728,17 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
     const int blk = first + W * i;
     const int pidx = block_page(a, blk);
     return static_cast<int64_t>(page) * a.page_stride +
-           static_cast<int64_t>((blk - pidx * bpp) * kBlock) * a.token_stride + static_cast<int64_t>(u.kvh) * D;
+           static_cast<int64_t>((blk - pidx * bpp) * kBlock) * a.token_stride + static_cast<int64_t>(cache_head) * D;
+  };
+  // PageScaled: a block's offset and its scales' index.
+  struct ScaledSrc {
+    int64_t off, scale;
+  };
+  struct BlockScales {
+    float k, v;
+  };
+  auto scaled_src = [&](int i, int page) {
+    return ScaledSrc{page_base(i, page), static_cast<int64_t>(page) * a.cache_heads + cache_head};
   };
   auto block_base = [&](int i) -> int64_t { return page_base(i, bt[block_page(a, first + W * i)]); };
   // The block-table entry of block i by a vector load (every lane reads the
@@ -790,12 +821,19 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
     if constexpr (SP) {
       return block_rows(i, entry);
     } else {
-      return page_base(i, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, entry)));
+      const int page = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, entry));
+      if constexpr (PS) {
+        return scaled_src(i, page);
+      } else {
+        return page_base(i, page);
+      }
     }
   };
   auto first_src = [&](int i) {
     if constexpr (SP) {
       return block_rows(i, entries_load(i));
+    } else if constexpr (PS) {
+      return scaled_src(i, bt[block_page(a, first + W * i)]);
     } else {
       return block_base(i);
     }
@@ -829,12 +867,20 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
       for (int c = 0; c < NL; ++c) vf[c] = buffer_load16<kKvPolicy>(vr, kv_off[c]);
     }
   };
-  // One 16-byte load's elements into a staging row as E: a plain store for a
-  // 16-bit cache, decoded to two 16-byte chunks for FP8.
-  auto stage16 = [&](S* dst, u32x4 v) {
+  // PageScaled: the loads of a block's scales, then its K and V, so that the wait
+  // for K covers the scales.
+  auto load_scaled = [&](const auto& src, u32x4 (&kf)[NL], u32x4 (&vf)[NL], BlockScales& sc, bool live) {
+    const int records = live ? 4 : 0;
+    sc.k = buffer_load_f32(make_rsrc_bytes(a.k_scale + src.scale, records), 0);
+    sc.v = buffer_load_f32(make_rsrc_bytes(a.v_scale + src.scale, records), 0);
+    load_block(src.off, kf, vf, live);
+  };
+  // One 16-byte load's elements into a staging row as X (E, or PE for V): a plain
+  // store for a 16-bit cache, decoded to two 16-byte chunks for FP8.
+  auto stage16 = [&](S* dst, u32x4 v, auto x) {
     if constexpr (KV8) {
       u32x4 lo, hi;
-      fp8x16_to<E>(v, lo, hi);
+      fp8x16_to<decltype(x)>(v, lo, hi);
       *reinterpret_cast<u32x4*>(dst) = lo;
       *reinterpret_cast<u32x4*>(dst + 8) = hi;
     } else {
@@ -846,8 +892,11 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
   // operand of S = K Q^T: lane holds token `row`, dims 32c + 8grp .. +7),
   // a stage_v(nvalid) step run before the V tiles are read, and v_tile(dt),
   // which reads V^T tile dt (lane holds V[token 4grp + j][dim 16dt + row]).
-  auto compute_block = [&](int i, const u32x4 (&ka)[KC], auto&& stage_v, auto&& v_tile, auto exact) {
+  // sc: the block's scales (PageScaled).
+  auto compute_block = [&](int i, const u32x4 (&ka)[KC], auto&& stage_v, auto&& v_tile, auto exact,
+                           const BlockScales& sc_blk = {}) {
     const int nvalid = valid_of(i);
+    const float qk_blk = PS ? qk_scale * sc_blk.k : qk_scale;
 
     // Scores: lane holds S[token 4grp + i][head row] for tile t.
     constexpr bool kExact = decltype(exact)::value;
@@ -887,7 +936,7 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
       }
       float sc[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sc[j] = s[j] * qk_scale;
+      for (int j = 0; j < 4; ++j) sc[j] = s[j] * qk_blk;
       // Only a sequence's last block (and a padding slot) has tokens to mask;
       // nvalid is wave-uniform, so full blocks skip the selects.
       if (nvalid < kBlock) {
@@ -939,8 +988,12 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
       if constexpr (kExact) {
         p32[t] = f32x4{p[0], p[1], p[2], p[3]};
       } else {
-        pf[t] = u32x2{pack2<E>(p[0], p[1]), pack2<E>(p[2], p[3])};
-        pl[t] = u32x2{pack2_residual<E>(p[0], p[1], pf[t][0]), pack2_residual<E>(p[2], p[3], pf[t][1])};
+        if constexpr (PS) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] *= sc_blk.v;
+        }
+        pf[t] = u32x2{pack2<PE>(p[0], p[1]), pack2<PE>(p[2], p[3])};
+        pl[t] = u32x2{pack2_residual<PE>(p[0], p[1], pf[t][0]), pack2_residual<PE>(p[2], p[3], pf[t][1])};
         if constexpr (kThirdPart) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -984,7 +1037,7 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
             acc[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[j], p32[t][j], acc[t][dt], 0, 0, 0);
           }
         } else {
-          acc[t][dt] = pv_split<E>(va, pf[t], pl[t], acc[t][dt]);
+          acc[t][dt] = pv_split<PE>(va, pf[t], pl[t], acc[t][dt]);
           // The third part by the same instruction: the compiler lets a
           // 16x16x16 product follow a 16x16x32 one on its accumulator sooner
           // than the hardware does (outputs lost the first one's).
@@ -996,10 +1049,11 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
 
   // Register pipeline: block i's K and V arrive in registers (kf, vf) and are
   // re-laid out through this wave's LDS tile.
-  auto process_block = [&](auto i, const u32x4 (&kf)[NL], const u32x4 (&vf)[NL], auto exact) {
+  auto process_block = [&](auto i, const u32x4 (&kf)[NL], const u32x4 (&vf)[NL], auto exact,
+                           const BlockScales& sc = {}) {
     // Stage K (its rows past seq_len only feed scores replaced by -inf).
 #pragma unroll
-    for (int c = 0; c < NL; ++c) stage16(kstage + load_tok(c) * KROW + load_dim(c), kf[c]);
+    for (int c = 0; c < NL; ++c) stage16(kstage + load_tok(c) * KROW + load_dim(c), kf[c], E{});
     u32x4 ka[KC];
 #pragma unroll
     for (int c = 0; c < KC; ++c) ka[c] = *reinterpret_cast<const u32x4*>(k_src + 4 * EPC * c);
@@ -1010,10 +1064,10 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
 #pragma unroll
           for (int c = 0; c < NL; ++c) {
             const int tok = load_tok(c);
-            stage16(stage + tok * VROW + load_dim(c), tok < nvalid ? vf[c] : u32x4{0, 0, 0, 0});
+            stage16(stage + tok * VROW + load_dim(c), tok < nvalid ? vf[c] : u32x4{0, 0, 0, 0}, PE{});
           }
         },
-        [&](int dt) { return lds_read_tr16(tr_src + 16 * dt); }, exact);
+        [&](int dt) { return lds_read_tr16(tr_src + 16 * dt); }, exact, sc);
   };
 
   // LDS pipeline: block i's K and V load straight into its LDS slot (rows
@@ -1104,7 +1158,7 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
         src = block_src(min(i + 1, nblk - 1), entry);
         entry = table_load(min(i + 2, nblk - 1));
 #pragma unroll
-        for (int c = 0; c < NL; ++c) stage16(kstage + load_tok(c) * KROW + load_dim(c), kf[c]);
+        for (int c = 0; c < NL; ++c) stage16(kstage + load_tok(c) * KROW + load_dim(c), kf[c], E{});
         load_half(kc, src, kf, more);
         u32x4 ka[KC];
 #pragma unroll
@@ -1150,8 +1204,16 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
     std::conditional_t<SP, Entries, float> pg[NS];
 #pragma unroll
     for (int k = NS - 1; k < 2 * NS - 1; ++k) pg[k % NS] = table_load(min(k, nblk - 1));
+    BlockScales sb[NS];
+    auto load_slot = [&](const auto& src, int slot, bool live) {
+      if constexpr (PS) {
+        load_scaled(src, kb[slot], vb[slot], sb[slot], live);
+      } else {
+        load_block(src, kb[slot], vb[slot], live);
+      }
+    };
 #pragma unroll
-    for (int s = 0; s < NS - 1; ++s) load_block(first_src(min(s, nblk - 1)), kb[s], vb[s], s < nblk);
+    for (int s = 0; s < NS - 1; ++s) load_slot(first_src(min(s, nblk - 1)), s, s < nblk);
     for (int base = 0; base < nblk; base += NS) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
@@ -1160,8 +1222,12 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
         const int j = min(i + NS - 1, nblk - 1);
         const auto next = block_src(j, pg[slot]);
         pg[slot] = table_load(min(i + 2 * NS - 1, nblk - 1));
-        load_block(next, kb[slot], vb[slot], i + NS - 1 < nblk);
-        process_block(i, kb[s], vb[s], std::false_type{});
+        load_slot(next, slot, i + NS - 1 < nblk);
+        if constexpr (PS) {
+          process_block(i, kb[s], vb[s], std::false_type{}, sb[s]);
+        } else {
+          process_block(i, kb[s], vb[s], std::false_type{});
+        }
       }
     }
     if constexpr (P32) {
@@ -3296,15 +3362,33 @@ extern "C" int kl_paged_decode_plan(kl_dtype dtype, int batch, int num_q_heads, 
 namespace kl {
 namespace {
 
-// Shared body of the two decode entry points. kv8: the caches hold OCP e4m3
-// codes with per-KV-head fp32 scales; otherwise they hold `dtype` like q.
-int decode_entry(kl_dtype dtype, bool kv8, void* out, const void* q, const void* k_cache, const void* v_cache,
+// What the caches hold: `dtype` like q, or OCP e4m3 codes with fp32 scales per KV
+// head, or per page and KV head, block tables per sequence or per (sequence, KV
+// head).
+enum class Cache { kSame, kHeadScales, kPageScales, kPageScalesHeadTables };
+
+// Shared body of the decode entry points. With block tables per KV head a
+// (sequence, KV head) pair is a sequence of one KV head to the planner and the
+// kernels, which take its head of the cache from its index (cache_head).
+int decode_entry(kl_dtype dtype, Cache cache, void* out, const void* q, const void* k_cache, const void* v_cache,
                  const float* k_scale, const float* v_scale, const int32_t* block_table, const int32_t* seq_lens,
                  int batch, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
                  int64_t block_table_stride, int max_pages, float scale, int num_splits, void* workspace,
                  size_t workspace_bytes, hipStream_t stream) {
   g_last_merge = KL_MERGE_NONE;
   if (batch == 0) return ok();
+  const bool kv8 = cache != Cache::kSame;
+  const int cache_heads = num_kv_heads;
+  if (cache == Cache::kPageScalesHeadTables) {
+    if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0) {
+      return fail(KL_ERR_INVALID_ARGUMENT, "batch and heads must be positive, num_q_heads a multiple of num_kv_heads");
+    }
+    const int64_t lists = static_cast<int64_t>(batch) * num_kv_heads;
+    if (lists > 0x7fffffffLL) return fail(KL_ERR_UNSUPPORTED, "too many (sequence, KV head) pairs");
+    batch = static_cast<int>(lists);
+    num_q_heads /= num_kv_heads;
+    num_kv_heads = 1;
+  }
   if (kv8) {
     if (dtype != KL_DTYPE_F16 && dtype != KL_DTYPE_BF16) {
       return fail(KL_ERR_UNSUPPORTED, "an FP8 cache needs fp16 or bf16 queries");
@@ -3351,10 +3435,12 @@ int decode_entry(kl_dtype dtype, bool kv8, void* out, const void* q, const void*
   a.o_part = static_cast<float*>(workspace);
   a.lse_part = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_bytes) : nullptr;
   a.bt_stride = block_table_stride;
-  a.page_stride = static_cast<int64_t>(page_size) * num_kv_heads * head_dim;
-  const int64_t token_stride = static_cast<int64_t>(num_kv_heads) * head_dim;
+  a.page_stride = static_cast<int64_t>(page_size) * cache_heads * head_dim;
+  const int64_t token_stride = static_cast<int64_t>(cache_heads) * head_dim;
   if (token_stride > 0x7fffffffLL / 64) return fail(KL_ERR_UNSUPPORTED, "num_kv_heads * head_dim too large");
   a.token_stride = static_cast<int>(token_stride);
+  a.cache_heads = cache_heads;
+  a.list_heads = cache == Cache::kPageScalesHeadTables ? cache_heads : 0;
   a.batch = batch;
   a.num_q_heads = num_q_heads;
   a.num_kv_heads = num_kv_heads;
@@ -3376,6 +3462,10 @@ int decode_entry(kl_dtype dtype, bool kv8, void* out, const void* q, const void*
   a.arrivals = nullptr;
 
   const bool small_pages = p.mfma && page_size % kBlock != 0;
+  if (cache == Cache::kPageScales || cache == Cache::kPageScalesHeadTables) {
+    return dtype == KL_DTYPE_F16 ? launch_typed<F16, PageScaled>(a, head_dim, true, stream)
+                                 : launch_typed<BF16, PageScaled>(a, head_dim, true, stream);
+  }
   switch (dtype) {
     case KL_DTYPE_F32:
       return small_pages ? launch_typed<F32, SmallPages<F32>>(a, head_dim, true, stream)
@@ -3400,7 +3490,7 @@ extern "C" int kl_paged_decode_attention(kl_dtype dtype, void* out, const void* 
                                          int batch, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
                                          int64_t block_table_stride, int max_pages, float scale, int num_splits,
                                          void* workspace, size_t workspace_bytes, kl_stream_t stream) {
-  return kl::decode_entry(dtype, false, out, q, k_cache, v_cache, nullptr, nullptr, block_table, seq_lens, batch,
+  return kl::decode_entry(dtype, kl::Cache::kSame, out, q, k_cache, v_cache, nullptr, nullptr, block_table, seq_lens, batch,
                           num_q_heads, num_kv_heads, head_dim, page_size, block_table_stride, max_pages, scale,
                           num_splits, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
@@ -3492,7 +3582,7 @@ extern "C" int kl_paged_decode_attention_noalloc(kl_dtype dtype, void* out, cons
                   need, kScratchBytes);
     return fail(KL_ERR_WORKSPACE, msg);
   }
-  return kl::decode_entry(dtype, false, out, q, k_cache, v_cache, nullptr, nullptr, block_table, seq_lens, batch,
+  return kl::decode_entry(dtype, kl::Cache::kSame, out, q, k_cache, v_cache, nullptr, nullptr, block_table, seq_lens, batch,
                           num_q_heads, num_kv_heads, head_dim, page_size, block_table_stride, max_pages, scale,
                           num_splits, need > 0 ? ws : nullptr, need > 0 ? kScratchBytes : 0,
                           reinterpret_cast<hipStream_t>(stream));
@@ -3505,9 +3595,22 @@ extern "C" int kl_paged_decode_attention_fp8(kl_dtype dtype, void* out, const vo
                                              int64_t block_table_stride, int max_pages, float scale,
                                              int num_splits, void* workspace, size_t workspace_bytes,
                                              kl_stream_t stream) {
-  return kl::decode_entry(dtype, true, out, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, batch,
+  return kl::decode_entry(dtype, kl::Cache::kHeadScales, out, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, batch,
                           num_q_heads, num_kv_heads, head_dim, page_size, block_table_stride, max_pages, scale,
                           num_splits, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int kl_paged_decode_attention_fp8_pages(kl_dtype dtype, void* out, const void* q, const void* k_cache,
+                                                   const void* v_cache, const float* k_scale, const float* v_scale,
+                                                   const int32_t* block_table, const int32_t* seq_lens, int batch,
+                                                   int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                                   int64_t block_table_stride, int max_pages, int head_tables,
+                                                   float scale, int num_splits, void* workspace,
+                                                   size_t workspace_bytes, kl_stream_t stream) {
+  return kl::decode_entry(dtype, head_tables ? kl::Cache::kPageScalesHeadTables : kl::Cache::kPageScales, out, q,
+                          k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, batch, num_q_heads, num_kv_heads,
+                          head_dim, page_size, block_table_stride, max_pages, scale, num_splits, workspace,
+                          workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
 // ------------------------------------------------------- cascade entry points

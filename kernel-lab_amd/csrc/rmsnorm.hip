@@ -26,14 +26,10 @@
 
 #include "hip_common.h"
 #include "kl_internal.h"
+#include "norm_rows.h"
 
 namespace kl {
 namespace {
-
-template <typename S, int N>
-struct alignas(sizeof(S) * N) Pack {
-  S v[N];
-};
 
 // Pack loads and stores keep the default cache policy: measured on MI355X for
 // this read/write mix, non-temporal stores lose ~10% of HBM bandwidth and
@@ -51,70 +47,6 @@ constexpr int kPacksPerThread = 2;
 template <typename S, int N>
 __device__ __forceinline__ void store_pack(Pack<S, N>* p, const Pack<S, N>& v) {
   *p = v;
-}
-
-constexpr int kMaxThreads = 1024;
-
-// Where x's rows are, in elements: row i of group g at g * group_stride + i *
-// row_stride, inner rows to a group; out and the residuals hold row g * inner +
-// i there. A strided view of two leading dimensions (the heads of one part of a
-// fused projection) is read in place; copied first, 2,048 x 32 heads of 128
-// bf16 took 15.7 us a call, the copy 9.7 of them, and 6.9 read in place (calls back
-// to back; the kernel alone traces at 7.3 with the profiler's gaps).
-//
-// A workgroup per row takes (i, g) from the grid, the larger of the two counts
-// along x: a division before the first load cost the large sizes 2 %.
-struct RowMap {
-  int64_t inner, row_stride, group_stride;
-  int swapped;  // the grid's x counts groups
-  __device__ __forceinline__ void of_workgroup(int64_t* row, int64_t* x_off) const {
-    const int64_t i = swapped ? blockIdx.y : blockIdx.x;
-    const int64_t g = swapped ? blockIdx.x : blockIdx.y;
-    *row = g * inner + i;
-    *x_off = g * group_stride + i * row_stride;
-  }
-  __device__ __forceinline__ int64_t x_of_row(int64_t r) const {
-    if (group_stride == 0) return r * row_stride;  // one group
-    const uint32_t g = static_cast<uint32_t>(r) / static_cast<uint32_t>(inner);
-    return g * group_stride + (r - g * inner) * row_stride;
-  }
-};
-
-__device__ __forceinline__ float inv_rms(float sum_sq, int hidden, float eps) {
-  // Division and square root are IEEE-rounded here (no fast-math), matching
-  // torch.rsqrt on the CPU, which computes 1 / sqrt(x).
-  return 1.0f / sqrtf(sum_sq / static_cast<float>(hidden) + eps);
-}
-
-// The new residual's place, `bytes` past the old one's: 0 in place. Reached
-// from the same pointer, so that pointer can be __restrict__ in both forms
-// (without it the large sizes lost 1 %: the weights' loads went ahead of the
-// residual's).
-template <typename S>
-__device__ __forceinline__ S* residual_out(S* res, int64_t bytes) {
-  return reinterpret_cast<S*>(reinterpret_cast<char*>(res) + bytes);
-}
-
-// The 16 bytes at element offset `off` of a row. Unaligned rows (any element
-// alignment) use the same 16-byte memory instructions, which gfx950 takes at
-// any address.
-template <bool ALIGNED, typename P, typename S>
-__device__ __forceinline__ P load_at(const S* row, int off) {
-  P v;
-  if constexpr (ALIGNED) {
-    v = *reinterpret_cast<const P*>(row + off);
-  } else {
-    __builtin_memcpy(&v, row + off, sizeof(P));
-  }
-  return v;
-}
-template <bool ALIGNED, typename P, typename S>
-__device__ __forceinline__ void store_at(S* row, int off, const P& v) {
-  if constexpr (ALIGNED) {
-    *reinterpret_cast<P*>(row + off) = v;
-  } else {
-    __builtin_memcpy(row + off, &v, sizeof(P));
-  }
 }
 
 // One thread's share of a row: packs t, t + nt, ..., NPACK of them, held in
@@ -186,18 +118,6 @@ __device__ __forceinline__ void norm_row(typename E::S* out, const typename E::S
     for (int j = 0; j < VEC; ++j) o.v[j] = E::from_f32((E::to_f32(a[k].v[j]) * rstd) * E::to_f32(w[k].v[j]));
     if (valid[k] && live) store_at<ALIGNED>(out, off[k], o);
   }
-}
-
-// Sum over the LANES (4 .. 64) lanes of a row, in every one of them.
-template <int LANES>
-__device__ __forceinline__ float lanes_sum(float v) {
-  v += dpp<kDppQuadSwap1>(v);
-  v += dpp<kDppQuadSwap2>(v);
-  if constexpr (LANES >= 8) v += dpp<kDppRowHalfMirror>(v);  // the quads of each half row agree, so a mirror is a swap
-  if constexpr (LANES >= 16) v += dpp<kDppRowRor8>(v);
-  if constexpr (LANES >= 32) v = sum_xor16(v);
-  if constexpr (LANES >= 64) v = sum_xor32(v);
-  return v;
 }
 
 // Workgroup-wide sum; every thread receives the same value. `scratch` holds one
@@ -434,8 +354,6 @@ __global__ void __launch_bounds__(kMaxThreads)
       res_out, weight, hidden, eps, threadIdx.x, blockDim.x, true, [&](float v) { return block_sum(v, scratch); });
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 // Calls f(IntC<N>) with the smallest N of 2, 4, 8 that holds npack (a row of one
 // pack per thread is narrow enough for rms_norm_rows_kernel).
 template <int N>
@@ -561,11 +479,7 @@ extern "C" int kl_rms_norm_grouped(kl_dtype dtype, void* out, const void* x, con
   const auto s = reinterpret_cast<hipStream_t>(stream);
   const int h = static_cast<int>(hidden);
   const int64_t rows = groups * rows_per_group;
-  // One row per group, or one group: a single stride. The grid's y is at most
-  // 65,535, which the smaller of two counts whose product is below 2^31 meets.
-  const RowMap xm = groups == 1           ? RowMap{rows, x_row_stride, 0, 0}
-                    : rows_per_group == 1 ? RowMap{rows, x_group_stride, 0, 0}
-                                          : RowMap{rows_per_group, x_row_stride, x_group_stride, groups > rows_per_group};
+  const RowMap xm = make_row_map(groups, rows_per_group, x_group_stride, x_row_stride);
   switch (dtype) {
     case KL_DTYPE_F32:
       return launch_any<F32>(out, x, residual, residual_out, weight, rows, h, xm, eps, s);

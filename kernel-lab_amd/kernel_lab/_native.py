@@ -57,6 +57,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i64, _i32, _f32, _i32, _vp, _sz, _vp],
     ),
+    "kl_rms_norm_fp8": (
+        _i32,
+        [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _vp],
+    ),
+    "kl_paged_decode_attention_fp8_pages": (
+        _i32,
+        [_i32, *[_vp] * 8, *[_i32] * 5, _i64, _i32, _i32, _f32, _i32, _vp, _sz, _vp],
+    ),
+    "kl_append_kv_fp8": (
+        _i32,
+        [_i32, *[_vp] * 7, *[_i64] * 4, _vp, _vp, _vp, _i64, *[_i32] * 5, _i64, _i32, _vp],
+    ),
+    "kl_select_pages_workspace": (_i32, [_i32, _i32, _i32, ctypes.POINTER(_sz)]),
+    "kl_select_pages": (
+        _i32,
+        [_i32, *[_vp] * 7, *[_i32] * 5, _i64, *[_i32] * 4, _vp, _sz, _vp],
+    ),
 }
 
 # kl_dtype / kl_status values from include/kernel_lab.h.

@@ -232,6 +232,51 @@ def quantize_fp8(kv: PagedKV) -> tuple[PagedKV, torch.Tensor, torch.Tensor]:
 
 
 @dataclass
+class PagedFP8:
+    """An FP8 cache with scales per page and KV head (``ops.append_kv_fp8``)."""
+
+    k_cache: torch.Tensor  # float8_e4m3fn [num_pages, page_size, num_kv_heads, head_dim]
+    v_cache: torch.Tensor
+    k_scale: torch.Tensor  # float32 [num_pages, num_kv_heads]
+    v_scale: torch.Tensor
+    k_bounds: torch.Tensor  # float8_e4m3fn [num_pages, num_kv_heads, 2, head_dim]: smallest, largest code
+    block_table: torch.Tensor
+    seq_lens: torch.Tensor
+    page_size: int
+
+
+def quantize_fp8_pages(kv: PagedKV) -> PagedFP8:
+    """The cache in OCP FP8 E4M3 with a float32 scale per page and KV head.
+
+    A page's scale is max |x| over the head's cached tokens on it / 448, at
+    least 2^-126; its codes are round-to-nearest-even(x / scale). Slots behind a
+    sequence's last token and spare pages become NaN codes, scales of spare pages NaN:
+    a correct kernel never reads them. ``k_bounds`` holds the smallest and
+    largest key code of each dimension over the page's tokens.
+    """
+    pages, page, heads, dim = kv.k_cache.shape
+    held = torch.zeros(pages, dtype=torch.int64, device=kv.k_cache.device)
+    for row, n in zip(kv.block_table.long(), kv.seq_lens.tolist()):
+        count = pages_for(n, page)
+        held[row[:count]] = page
+        if n % page:
+            held[row[count - 1]] = n % page
+    live = (torch.arange(page, device=held.device)[None, :] < held[:, None])[:, :, None, None]
+    codes, scales = [], []
+    for cache in (kv.k_cache, kv.v_cache):
+        x = torch.where(live, cache.float(), torch.zeros((), device=held.device))
+        scale = (x.abs().amax(dim=(1, 3)) / FP8_E4M3_MAX).clamp(min=2.0**-126)
+        c = torch.where(live, x / scale[:, None, :, None], torch.full((), float("nan"), device=held.device))
+        codes.append(c.to(torch.float8_e4m3fn))
+        scales.append(torch.where(held[:, None] > 0, scale, torch.full_like(scale, float("nan"))))
+    k = codes[0].float()
+    bounds = torch.stack([k.nan_to_num(nan=FP8_E4M3_MAX).amin(1), k.nan_to_num(nan=-FP8_E4M3_MAX).amax(1)], 2)
+    return PagedFP8(
+        codes[0], codes[1], scales[0], scales[1], bounds.to(torch.float8_e4m3fn), kv.block_table, kv.seq_lens, page
+    )
+
+
+@dataclass
 class CascadeKV:
     """A paged pool holding a shared prefix and each sequence's own tokens."""
 

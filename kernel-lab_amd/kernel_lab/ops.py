@@ -112,6 +112,82 @@ def fused_add_rms_norm_(
     return out
 
 
+# -------------------------------------------------- RMSNorm with an FP8 output
+
+FP8_SCALE_GROUPS = (32, 64, 128, 256)
+
+
+def _fp8_outputs(x: torch.Tensor, group_size: int | None) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """Empty codes and scales for x, and the operator's scale_group."""
+    hidden = x.shape[-1]
+    group = 0 if group_size is None or group_size == hidden else int(group_size)
+    if group and group not in FP8_SCALE_GROUPS:
+        raise ValueError(f"group_size must be None (a scale per row) or one of {FP8_SCALE_GROUPS}, got {group_size}")
+    if group and hidden % group:
+        raise ValueError(f"hidden size {hidden} is not a multiple of group_size {group}")
+    out = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((*x.shape[:-1], hidden // group if group else 1), dtype=torch.float32, device=x.device)
+    return out, scales, group
+
+
+def rms_norm_fp8(
+    x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, group_size: int | None = None
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``rms_norm`` with an FP8 output: (codes, scales), the input of an 8-bit projection.
+
+    With y = x / sqrt(mean(x^2) + eps) * weight in float32, ``scales`` is
+    max |y| / 448 (at least 2^-126) over each row ([..., 1]) or over each
+    ``group_size`` (32, 64, 128 or 256) consecutive columns ([..., hidden /
+    group_size]), and the float8_e4m3fn codes are y / scale rounded to nearest
+    even. A y that is not finite becomes a NaN code and does not count towards
+    its scale.
+    """
+    _check_rms(x, weight, None)
+    _native.require_ops()
+    x = _rows_view(x)
+    out, scales, group = _fp8_outputs(x, group_size)
+    torch.ops.kernel_lab.rms_norm_fp8(out, scales, x, weight.contiguous(), eps, group)
+    return out, scales
+
+
+def fused_add_rms_norm_fp8(
+    x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, group_size: int | None = None
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``fused_add_rms_norm`` with an FP8 output (``rms_norm_fp8``): returns
+    (codes, scales, new_residual) and leaves ``residual`` untouched."""
+    _check_rms(x, weight, residual)
+    _native.require_ops()
+    x = _rows_view(x)
+    out, scales, group = _fp8_outputs(x, group_size)
+    residual = residual.contiguous()
+    if _carries_nothing(residual):
+        new_residual = torch.empty_like(residual)
+        torch.ops.kernel_lab.fused_add_rms_norm_fp8_new(
+            out, scales, new_residual, x, residual, weight.contiguous(), eps, group
+        )
+    else:
+        new_residual = residual.clone()
+        torch.ops.kernel_lab.fused_add_rms_norm_fp8(out, scales, x, new_residual, weight.contiguous(), eps, group)
+    return out, scales, new_residual
+
+
+def fused_add_rms_norm_fp8_(
+    x: torch.Tensor,
+    residual: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float = 1e-6,
+    group_size: int | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """In-place pre-norm step: residual += x (rounded to its dtype), returns
+    (codes, scales) of rmsnorm(residual) as ``rms_norm_fp8`` does."""
+    _check_rms(x, weight, residual)
+    _native.require_ops()
+    x = _rows_view(x)
+    out, scales, group = _fp8_outputs(x, group_size)
+    torch.ops.kernel_lab.fused_add_rms_norm_fp8(out, scales, x, residual, weight, eps, group)
+    return out, scales
+
+
 # ---------------------------------------------------------- decode attention
 
 
@@ -157,6 +233,12 @@ def paged_decode_attention(
     ``v_scale`` (one float32 per KV head, or one float for all) give head h's
     values as ``k_scale[h] * k`` and ``v_scale[h] * v``. q is then float16 or
     bfloat16 and the output has q's dtype.
+
+    Scales of shape [num_pages, num_kv_heads] are per page and KV head, as
+    ``append_kv_fp8`` keeps them. With them ``block_table`` may be [batch,
+    num_kv_heads, pages] and ``seq_lens`` [batch, num_kv_heads], a table and a
+    length for each (sequence, KV head): sparse decode over the pages that
+    ``select_pages`` chose.
     """
     _check_decode(q, k_cache, v_cache)
     _native.require_ops()
@@ -168,6 +250,17 @@ def paged_decode_attention(
         if k_scale is None or v_scale is None:
             raise ValueError("an FP8 cache needs k_scale and v_scale")
         hkv = k_cache.shape[2]
+        # One page's [1, num_kv_heads] scales are scales per head.
+        if block_table.dim() == 3 or (k_cache.shape[0] > 1 and _page_scales(k_scale, k_cache)):
+            if not (_page_scales(k_scale, k_cache) and _page_scales(v_scale, k_cache)):
+                raise ValueError("k_scale and v_scale must both be [num_pages, num_kv_heads]")
+            if block_table.dim() == 3:
+                block_table, seq_lens = block_table.contiguous(), seq_lens.contiguous()
+            torch.ops.kernel_lab.paged_decode_attention_fp8_pages(
+                out, q, k_cache, v_cache, block_table, seq_lens, scale, k_scale, v_scale, int(num_splits or 0),
+                int(max_seq_len or 0),
+            )
+            return out
         ks = _head_scales(k_scale, hkv, q.device)
         vs = _head_scales(v_scale, hkv, q.device)
         torch.ops.kernel_lab.paged_decode_attention_fp8(
@@ -218,6 +311,101 @@ def cascade_decode_attention(
         out, q, k_cache, v_cache, prefix_block_table, prefix_len.reshape(1), block_table, seq_lens, scale
     )
     return out
+
+
+def _page_scales(s: torch.Tensor | float, cache: torch.Tensor) -> bool:
+    return isinstance(s, torch.Tensor) and s.dim() == 2 and s.shape == (cache.shape[0], cache.shape[2])
+
+
+def append_kv_fp8(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    new_offsets: torch.Tensor | None = None,
+    k_bounds: torch.Tensor | None = None,
+) -> None:
+    """Writes new keys and values into a paged FP8 cache, in place.
+
+    ``k`` and ``v`` are [tokens, num_kv_heads, head_dim] (float32, float16 or
+    bfloat16; a part of a fused projection is read in place). ``seq_lens``
+    counts the new tokens, which take the last positions of their sequences:
+    one token each, or with ``new_offsets`` (int32 [batch + 1]) rows
+    ``new_offsets[b] : new_offsets[b + 1]`` for sequence b. The caches are
+    float8_e4m3fn [num_pages, page_size, num_kv_heads, head_dim], ``k_scale``
+    and ``v_scale`` float32 [num_pages, num_kv_heads].
+
+    A page's scale is max |x| / 448 (at least 2^-126) over the finite values of
+    its tokens. A page that holds earlier tokens keeps its scale unless a new
+    token needs a larger one; then its codes are rounded again to that. Values
+    that are not finite become NaN codes. ``k_bounds`` (float8_e4m3fn
+    [num_pages, num_kv_heads, 2, head_dim]), if given, is kept as the smallest
+    and largest code of each page's keys in each dimension, which
+    ``select_pages`` reads.
+
+    A sequence whose length is less than its new tokens is left alone (give
+    the idle rows of a padded batch length 0), and so are tokens whose page is
+    outside the table or the cache. Two sequences must not append to the same
+    page in one call. The result is a cache, not a function of ``k`` and ``v``:
+    no gradient passes through it.
+    """
+    _native.require_ops()
+    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("k and v are [tokens, kv_heads, head_dim] and the caches [pages, page_size, kv_heads, head_dim]")
+    if k.shape[1:] != k_cache.shape[2:]:
+        raise ValueError(f"k is {tuple(k.shape)} but the cache has heads {tuple(k_cache.shape[2:])}")
+    if new_offsets is None and k.shape[0] != seq_lens.shape[0]:
+        raise ValueError("without new_offsets, k and v have one token per sequence")
+    torch.ops.kernel_lab.append_kv_fp8(
+        _rows_view(k), _rows_view(v), k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, new_offsets, k_bounds
+    )
+
+
+def select_pages(
+    q: torch.Tensor,
+    k_bounds: torch.Tensor,
+    k_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    num_pages: int,
+    page_size: int,
+    first_pages: int = 1,
+    last_pages: int = 1,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Chooses the pages that each (sequence, KV head) attends: (table, lens).
+
+    A page's score is k_scale * max over the KV head's query heads of
+    sum_d max(q_d lo_d, q_d hi_d), with lo and hi from ``k_bounds``: no key of
+    the page has a larger q.k. It is summed in 64 bits and rounded to float32;
+    a NaN counts as the largest finite score. The sequence's first
+    ``first_pages`` and last ``last_pages`` (at least one) pages are kept in any
+    case, then those of the largest scores, equal ones lowest page first, up to
+    ``num_pages``; all of a sequence that has no more.
+
+    ``table`` (int32 [batch, num_kv_heads, num_pages], ids from ``block_table``
+    in the order of the sequence, padded with 0) and ``lens`` (int32 [batch,
+    num_kv_heads], the tokens on them) are what ``paged_decode_attention`` takes
+    with scales per page.
+    """
+    _native.require_ops()
+    if q.dim() != 3 or k_bounds.dim() != 4:
+        raise ValueError("q is [batch, heads, head_dim] and k_bounds [pages, kv_heads, 2, head_dim]")
+    num_kv_heads = k_bounds.shape[1]
+    if num_kv_heads < 1 or q.shape[1] % num_kv_heads:
+        raise ValueError("num_q_heads must be a multiple of num_kv_heads")
+    if first_pages < 0 or last_pages < 1 or first_pages + last_pages > num_pages:
+        raise ValueError("first_pages >= 0 and last_pages >= 1 must fit num_pages")
+    table = torch.empty((q.shape[0], num_kv_heads, num_pages), dtype=torch.int32, device=q.device)
+    lens = torch.empty((q.shape[0], num_kv_heads), dtype=torch.int32, device=q.device)
+    torch.ops.kernel_lab.select_pages(
+        table, lens, q.contiguous(), k_bounds, k_scale, block_table, seq_lens, int(page_size), int(first_pages),
+        int(last_pages),
+    )
+    return table, lens
 
 
 def _head_scales(s: torch.Tensor | float, num_kv_heads: int, device: torch.device) -> torch.Tensor:

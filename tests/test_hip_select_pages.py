@@ -1,0 +1,203 @@
+"""gfx950 page selection against the float64 oracle: tables and lengths have to be equal.
+
+The scores' sums are exact in 64 bits for these inputs on both sides (a product of a query and a code has at most 15 bits
+and the values' exponents span less than 30 binades), so their order does not matter, and both round once to float32.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from kernel_lab import _native
+from oracle import fp8_step as ref
+
+pytestmark = pytest.mark.gpu
+
+F8 = torch.float8_e4m3fn
+
+
+def problem(lens, hq, hkv, dim, dtype, page, seed=0, spare=5):
+    """Queries, bounds (smallest <= largest code, mixed signs), scales and a table of distinct pages."""
+    g = torch.Generator().manual_seed(seed)
+    need = [(max(n, 0) + page - 1) // page for n in lens]
+    total = sum(need) + spare
+    order = torch.randperm(total, generator=g).to(torch.int32)
+    table = torch.zeros(len(lens), max([*need, 1]), dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at : at + n]
+        at += n
+    edges = (100 * torch.randn(total, hkv, 2, dim, generator=g)).clamp(-448, 448).sort(2).values.to(F8)
+    scale = 0.01 * torch.exp(0.3 * torch.randn(total, hkv, generator=g))
+    spare_ids = order[at:].long()
+    edges.view(torch.uint8)[spare_ids] = 0x7F  # NaN
+    scale[spare_ids] = float("nan")
+    q = torch.randn(len(lens), hq, dim, generator=g).to(dtype)
+    return q, edges, scale, table, torch.tensor(lens, dtype=torch.int32)
+
+
+def check(ops, q, edges, scale, table, lens, keep, page, first=1, last=1):
+    got = ops.select_pages(q.cuda(), edges.cuda(), scale.cuda(), table.cuda(), lens.cuda(), keep, page, first_pages=first, last_pages=last)
+    want = ref.select(q, edges, scale, table, lens, keep, page, first, last)
+    assert torch.equal(got[1].cpu(), want[1])
+    assert torch.equal(got[0].cpu(), want[0]), (got[0].cpu() != want[0]).nonzero()[:5]
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize(("hq", "hkv"), [(8, 8), (16, 4), (8, 1), (32, 8), (32, 1), (12, 4), (80, 2)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_shapes(gpu_ops, hq, hkv, dim, dtype):
+    lens = [1, 16, 17, 160, 161, 333, 0, 2000]
+    check(gpu_ops, *problem(lens, hq, hkv, dim, dtype, 16, seed=dim), 10, 16)
+
+
+@pytest.mark.parametrize("keep", [1, 2, 3, 7, 64, 255, 256, 257, 500, 700])
+def test_keep_counts_on_long_tables(gpu_ops, keep):
+    check(gpu_ops, *problem([16 * 600 - 3, 16 * 256, 16 * 257, 5, 16 * 300 + 1], 16, 2, 128, torch.bfloat16, 16), keep, 16, first=0)
+
+
+@pytest.mark.parametrize(("first", "last"), [(0, 1), (1, 1), (0, 8), (7, 1), (4, 4), (3, 2)])
+def test_pinned_pages(gpu_ops, first, last):
+    check(gpu_ops, *problem([32 * 40, 32 * 8, 32 * 9, 32 * 3 + 1, 32], 8, 2, 64, torch.float16, 32, seed=3), 8, 32, first, last)
+
+
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 128])
+def test_page_sizes(gpu_ops, page):
+    check(gpu_ops, *problem([page * 33 + 7, page * 20, 3], 16, 4, 128, torch.bfloat16, page), 12, page)
+
+
+def test_equal_scores_take_the_lowest_pages(gpu_ops):
+    q, edges, scale, table, lens = problem([16 * 700], 8, 2, 128, torch.float16, 16)
+    edges.copy_(edges[:1].float().nan_to_num(0).to(F8).expand_as(edges))
+    scale.fill_(0.5)
+    check(gpu_ops, q, edges, scale, table, lens, 100, 16)
+    scale[table[0, 300:350].long()] = 0.75  # a run of better (or, below zero, worse) ones
+    check(gpu_ops, q, edges, scale, table, lens, 100, 16)
+    check(gpu_ops, -q, edges, scale, table, lens, 30, 16)
+    check(gpu_ops, torch.zeros_like(q), edges, scale, table, lens, 300, 16)
+
+
+def test_scores_below_zero_and_signed_zeros(gpu_ops):
+    q, edges, scale, table, lens = problem([16 * 90], 4, 1, 64, torch.bfloat16, 16)
+    q = q.abs()
+    edges = (-edges.float().nan_to_num(0).abs()).to(F8)
+    edges[:, :, 1] = edges[:, :, 0]
+    edges[table[0, 10:20].long()] = 0
+    edges.view(torch.uint8)[table[0, 20:30].long()] = 0x80  # -0
+    check(gpu_ops, q, edges, scale, table, lens, 12, 16)
+    check(gpu_ops, q, edges, scale, table, lens, 40, 16)
+
+
+def test_scores_that_are_not_numbers(gpu_ops):
+    """NaN and infinite scores count as the largest finite one; an infinite query, too."""
+    q, edges, scale, table, lens = problem([16 * 64, 16 * 64], 8, 2, 64, torch.bfloat16, 16)
+    scale[table[0, 20].long()] = float("nan")
+    scale[table[0, 30].long()] = float("inf")
+    edges.view(torch.uint8)[table[0, 40].long(), :, :, 5] = 0x7F
+    check(gpu_ops, q, edges, scale, table, lens, 6, 16)
+    q[1, 0, 3] = float("inf")
+    q[1, 5, 3] = float("nan")
+    check(gpu_ops, q, edges, scale, table, lens, 6, 16)
+
+
+def test_near_scores_are_told_apart(gpu_ops):
+    """Pages whose scores differ only behind the 24 bits that a float32 sum keeps at its size, but not once rounded."""
+    dim, pages = 128, 200
+    q = torch.full((1, 1, dim), 1.0, dtype=torch.float16)
+    q[..., 0] = 2.0**-14
+    edges = torch.zeros(pages, 1, 2, dim)
+    edges[..., 1:65], edges[..., 65:] = 448.0, -448.0  # they cancel
+    g = torch.Generator().manual_seed(0)
+    edges[..., 0] = torch.randint(1, 16, (pages, 1, 1), generator=g) * 1.0
+    table = torch.arange(pages, dtype=torch.int32)[None]
+    edges = edges.to(F8)
+    check(gpu_ops, q, edges, torch.ones(pages, 1), table, torch.tensor([16 * pages], dtype=torch.int32), 20, 16, first=0)
+
+
+def test_lengths_past_the_table_and_below_zero(gpu_ops):
+    q, edges, scale, table, lens = problem([16 * 30, 16 * 30, 16 * 30], 8, 2, 64, torch.bfloat16, 16)
+    lens = torch.tensor([16 * 30 + 100, -5, 2**31 - 1], dtype=torch.int32)
+    check(gpu_ops, q, edges, scale, table, lens, 8, 16)
+
+
+def test_strided_table(gpu_ops):
+    q, edges, scale, table, lens = problem([16 * 30, 40], 8, 2, 64, torch.bfloat16, 16)
+    wide = torch.full((2, 50), 1 << 29, dtype=torch.int32)
+    wide[:, : table.shape[1]] = table
+    got = gpu_ops.select_pages(q.cuda(), edges.cuda(), scale.cuda(), wide.cuda()[:, : table.shape[1]], lens.cuda(), 8, 16)
+    want = ref.select(q, edges, scale, table, lens, 8, 16)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
+def test_many_rows(gpu_ops):
+    lens = torch.randint(0, 1500, (130,), generator=torch.Generator().manual_seed(1)).tolist()
+    check(gpu_ops, *problem(lens, 32, 8, 64, torch.float16, 32), 16, 32, first=1, last=2)
+
+
+def test_empty_batch(gpu_ops):
+    q, edges, scale, table, lens = problem([16], 8, 2, 64, torch.bfloat16, 16)
+    got = gpu_ops.select_pages(q[:0].cuda(), edges.cuda(), scale.cuda(), table[:0].cuda(), lens[:0].cuda(), 8, 16)
+    assert got[0].shape == (0, 2, 8) and got[1].shape == (0, 2)
+
+
+def test_refusals(gpu_ops):
+    q, edges, scale, table, lens = (t.cuda() for t in problem([16 * 30], 8, 2, 64, torch.bfloat16, 16))
+    for bad in [{"first_pages": -1}, {"last_pages": 0}, {"first_pages": 5, "last_pages": 4}]:
+        with pytest.raises(ValueError, match="must fit"):
+            gpu_ops.select_pages(q, edges, scale, table, lens, 8, 16, **bad)
+    with pytest.raises(ValueError, match="multiple"):
+        gpu_ops.select_pages(q[:, :7], edges, scale, table, lens, 8, 16)
+    with pytest.raises(RuntimeError, match="multiple of 16"):
+        gpu_ops.select_pages(q, edges, scale, table, lens, 8, 8)
+    with pytest.raises(RuntimeError, match="float16 or bfloat16"):
+        gpu_ops.select_pages(q.float(), edges, scale, table, lens, 8, 16)
+    with pytest.raises(RuntimeError, match="k_scale"):
+        gpu_ops.select_pages(q, edges, scale[:-1], table, lens, 8, 16)
+    with pytest.raises(RuntimeError, match="k_bounds"):
+        gpu_ops.select_pages(q, edges.view(torch.uint8), scale, table, lens, 8, 16)
+    with pytest.raises(RuntimeError, match="one row per sequence"):
+        gpu_ops.select_pages(q, edges, scale, table, lens.repeat(2), 8, 16)
+
+
+def test_graph_replays(gpu_ops):
+    q, edges, scale, table, lens = (t.cuda() for t in problem([16 * 90, 16 * 300, 3], 16, 4, 128, torch.bfloat16, 16))
+    run = lambda: gpu_ops.select_pages(q, edges, scale, table, lens, 24, 16)  # noqa: E731
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for seed in range(4):
+        new = problem([16 * 90, 16 * 300, 3], 16, 4, 128, torch.bfloat16, 16, seed=seed)
+        for t, n in zip((q, edges, scale, table), new):
+            t.copy_(n)
+        lens.copy_(torch.tensor([16 * 90 - seed, 16 * (100 + seed), 3 + seed], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = ref.select(*(t.cpu() for t in (q, edges, scale, table, lens)), 24, 16)
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
+def test_through_c_abi(gpu_ops):
+    lib = _native.core()
+    host = problem([16 * 90, 16 * 40 + 3], 16, 4, 128, torch.bfloat16, 16)
+    q, edges, scale, table, lens = (t.cuda() for t in host)
+    ws = ctypes.c_size_t(0)
+    assert lib.kl_select_pages_workspace(2, 4, 90, ctypes.byref(ws)) == 0 and ws.value >= 2 * 4 * 90 * 4
+    work = torch.empty(ws.value, dtype=torch.uint8, device="cuda")
+    out, out_lens = torch.empty(2, 4, 12, dtype=torch.int32, device="cuda"), torch.empty(2, 4, dtype=torch.int32, device="cuda")
+
+    def call(bytes_=ws.value, first=1):
+        return lib.kl_select_pages(2, out.data_ptr(), out_lens.data_ptr(), q.data_ptr(), edges.data_ptr(), scale.data_ptr(),
+                                   table.data_ptr(), lens.data_ptr(), 2, 16, 4, 128, 16, 90, 90, 12, first, 1, work.data_ptr(),
+                                   bytes_, torch.cuda.current_stream().cuda_stream)
+
+    assert call() == 0, _native.last_error()
+    torch.cuda.synchronize()
+    want = ref.select(*host, 12, 16)
+    assert torch.equal(out.cpu(), want[0]) and torch.equal(out_lens.cpu(), want[1])
+    assert call(bytes_=ws.value - 4) == 3
+    assert call(first=12) == 1
