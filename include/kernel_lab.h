@@ -109,7 +109,8 @@ int kl_rms_norm_grouped(kl_dtype dtype, void* out, const void* x, const void* re
  *
  *   y      = rmsnorm(x) * weight, or of the new residual; fp32, not rounded to
  *            the input's type first
- *   scales = max(max |y| / 448, 2^-126) over the finite y of a scale group:
+ *   scales = max(max |y| / 448, 2^-126) over the finite y (whose x * weight is
+ *            finite) of a scale group:
  *            scale_group consecutive columns (32, 64, 128 or 256, dividing
  *            hidden), or the row (scale_group 0 or hidden)
  *   out    = e4m3(y / scale), round to nearest even; a y that is not finite

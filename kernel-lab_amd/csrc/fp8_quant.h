@@ -2,6 +2,7 @@
 #pragma once
 
 #include "hip_common.h"
+#include "packs.h"
 
 namespace kl {
 
@@ -32,9 +33,26 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return e4m3x2<true>(c, d, e4m3x2<false>(a, b, 0));
 }
 
+// The value of byte N of a word of codes.
+template <int N>
+__device__ __forceinline__ float e4m3_value_at(uint32_t word) {
+  return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(word), N);
+}
+
 // The value of a code.
-__device__ __forceinline__ float e4m3_value(uint32_t code) {
-  return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(code), 0);
+__device__ __forceinline__ float e4m3_value(uint32_t code) { return e4m3_value_at<0>(code); }
+
+// The codes of VEC values.
+template <bool ALIGNED, int VEC>
+__device__ __forceinline__ void store_codes(uint8_t* row, int off, const float (&c)[VEC]) {
+  static_assert(VEC == 4 || VEC == 8, "a pack is four or eight elements");
+  if constexpr (VEC == 8) {
+    const u32x2 v = {e4m3x4(c[0], c[1], c[2], c[3]), e4m3x4(c[4], c[5], c[6], c[7])};
+    store_at<ALIGNED>(row, off, v);
+  } else {
+    const uint32_t v = e4m3x4(c[0], c[1], c[2], c[3]);
+    store_at<ALIGNED>(row, off, v);
+  }
 }
 
 }  // namespace kl

@@ -1,16 +1,12 @@
-// What the RMSNorm kernels share: where a call's rows lie, packs of elements at
-// any alignment, and sums over a row's lanes.
+// What the RMSNorm kernels share: where a call's rows lie, and sums over a row's
+// lanes.
 #pragma once
 
 #include "hip_common.h"
+#include "packs.h"
 
 namespace kl {
 namespace {
-
-template <typename S, int N>
-struct alignas(sizeof(S) * N) Pack {
-  S v[N];
-};
 
 constexpr int kMaxThreads = 1024;
 
@@ -61,28 +57,6 @@ __device__ __forceinline__ float inv_rms(float sum_sq, int hidden, float eps) {
 template <typename S>
 __device__ __forceinline__ S* residual_out(S* res, int64_t bytes) {
   return reinterpret_cast<S*>(reinterpret_cast<char*>(res) + bytes);
-}
-
-// The 16 bytes at element offset `off` of a row. Unaligned rows (any element
-// alignment) use the same 16-byte memory instructions, which gfx950 takes at
-// any address.
-template <bool ALIGNED, typename P, typename S>
-__device__ __forceinline__ P load_at(const S* row, int off) {
-  P v;
-  if constexpr (ALIGNED) {
-    v = *reinterpret_cast<const P*>(row + off);
-  } else {
-    __builtin_memcpy(&v, row + off, sizeof(P));
-  }
-  return v;
-}
-template <bool ALIGNED, typename P, typename S>
-__device__ __forceinline__ void store_at(S* row, int off, const P& v) {
-  if constexpr (ALIGNED) {
-    *reinterpret_cast<P*>(row + off) = v;
-  } else {
-    __builtin_memcpy(row + off, &v, sizeof(P));
-  }
 }
 
 // Sum over the LANES (4 .. 64) lanes of a row, in every one of them.
