@@ -11,6 +11,7 @@
 #include "fp8_quant.h"
 #include "hip_common.h"
 #include "kl_internal.h"
+#include "packs.h"
 
 namespace kl {
 namespace {
@@ -37,11 +38,13 @@ struct AppendArgs {
   const int32_t* seq_lens;
   const int32_t* offsets;  // null: one token a sequence
   int tokens, batch, heads, dim, page, max_pages, num_pages;
+  int unit_blocks;  // workgroups a tile
 };
 
-// What a workgroup writes: new tokens [t0, t1) of a page, from row `row` on.
+// What a workgroup writes: new tokens [t0, t1) of a page, from row `row` on. The page
+// is as the table has it, in range or not.
 struct PageTile {
-  int64_t phys;
+  int phys;
   int t0, t1;
   int64_t row;
 };
@@ -50,101 +53,337 @@ struct PageTile {
 // them sequence b has the tiles from offsets[b] / page + 2 b on, one for each
 // page it reaches: n tokens reach at most n / page + 2 pages, so the next
 // sequence's first tile lies behind its last. False where the tile has no
-// tokens, and for sequences whose lengths, offsets or pages are out of range,
-// which are left alone.
+// tokens, and for sequences whose lengths or offsets are out of range, which are
+// left alone. Wave-uniform: the sequence is found by all lanes at once,
+// 64 offsets at a time.
 __device__ __forceinline__ bool page_tile(const AppendArgs& a, int i, PageTile* t) {
   int b = i, off = i, n = 1, at = 0;
   if (a.offsets != nullptr) {
-    int lo = 0, hi = a.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.offsets[mid] / a.page + 2 * mid <= i) {
-        lo = mid;
-      } else {
-        hi = mid - 1;
-      }
+    int before = 0;  // sequences whose first tile is not behind this one
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      const int s = b0 + __lane_id();
+      const bool reached = s < a.batch && a.offsets[s] / a.page + 2 * static_cast<int64_t>(s) <= i;
+      const int count = __builtin_popcountll(__ballot(reached));
+      before += count;
+      if (count < 64) break;
     }
-    b = lo;
-    off = a.offsets[b];
-    const int end = a.offsets[b + 1];
+    b = before > 0 ? before - 1 : 0;
+    off = as_constant(a.offsets)[b];
+    const int end = as_constant(a.offsets)[b + 1];
     if (off < 0 || end > a.tokens || end <= off) return false;
     n = end - off;
     at = i - (off / a.page + 2 * b);
   }
-  const int len = a.seq_lens[b];
+  const int len = as_constant(a.seq_lens)[b];
   const int start = len - n;
   if (start < 0 || at < 0) return false;
   const int64_t col = start / a.page + static_cast<int64_t>(at);
   if (col * a.page >= len || col >= a.max_pages) return false;
-  const int phys = a.table[b * a.bt_stride + col];
-  if (phys < 0 || phys >= a.num_pages) return false;
   const int64_t base = col * a.page;
-  t->phys = phys;
+  t->phys = as_constant(a.table)[b * a.bt_stride + col];
   t->t0 = static_cast<int>(max(static_cast<int64_t>(start) - base, static_cast<int64_t>(0)));
   t->t1 = static_cast<int>(min(static_cast<int64_t>(len) - base, static_cast<int64_t>(a.page)));
   t->row = off + (base + t->t0 - start);
   return true;
 }
 
-__device__ __forceinline__ float wave_max(float v) { return max_xor32(max_xor16(row16_max(v))); }
+// x / scale for many x of one scale, correctly rounded. Markstein's: a product with
+// the rounded reciprocal, and one step that adds its remainder; with a correctly
+// rounded reciprocal the result is the division's, in four instructions instead of
+// ten. The remainder has to be exact, so scale and x are first moved from the ends of
+// fp32's range by a power of two. An x that is not finite gives NaN.
+struct Over {
+  float pre, scale, inv;
+  __device__ __forceinline__ explicit Over(float s) {
+    pre = s < 0x1p-90f ? 0x1p100f : s > 0x1p90f ? 0x1p-100f : 1.0f;
+    scale = s * pre;
+    inv = 1.0f / scale;
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    x *= pre;
+    const float q = x * inv;
+    return fmaf(fmaf(-q, scale, x), inv, q);
+  }
+};
 
-constexpr int kAppendThreads = 256;
+// The smaller of x in this lane and the lane 32 (16) below or above it, in the lower
+// half (even rows), and of y in the upper half (odd rows): v_permlane32_swap
+// exchanges x's upper half with y's lower one.
+__device__ __forceinline__ float min_swap32(float x, float y) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+  return fminf(__builtin_bit_cast(float, static_cast<unsigned>(r[0])), __builtin_bit_cast(float, static_cast<unsigned>(r[1])));
+}
+__device__ __forceinline__ float min_swap16(float x, float y) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+  return fminf(__builtin_bit_cast(float, static_cast<unsigned>(r[0])), __builtin_bit_cast(float, static_cast<unsigned>(r[1])));
+}
 
-// A workgroup per (tile, KV head, K or V), element by element.
-template <typename E>
+// f, or NaN where it is infinite: the minimum and maximum instructions pass over it.
+__device__ __forceinline__ float finite_or_nan(float f) { return fmaf(f, 0.0f, f); }
+
+constexpr int kAppendWaves = 4;
+constexpr int kAppendThreads = kAppendWaves * 64;
+
+// A wave per (tile, KV head, K or V). A lane holds 16-byte packs of the tile's
+// tokens: the LPT lanes of a token read its head_dim contiguously, TPI tokens to a
+// load. Up to HOLD packs a lane stay in registers between the page's largest
+// magnitude and its codes; a longer tile is read again.
+//
+// What bounds it: HBM for prompts (3 bytes an element of 16 bits), the launch for
+// single tokens. Measured (us, 8 chunks of 2,048 .. 4,096 tokens, 8 heads of 128 bf16
+// read from a fused projection, pages of 16, with bounds): 35.8 (4.5 TB/s), element by
+// element 181; IEEE divisions and every lane reducing all bounds 53.5; K and V in
+// workgroups of their own 42.3 (K's are longer, and the XCDs take workgroups in
+// turn); tiles of one head group far apart in the launch 43.5; default-policy loads 3 to
+// 10 % more; four heads one after the other in a wave, the next one loading, 51.
+template <typename E, int D, int HOLD, bool ALIGNED>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
   using S = typename E::S;
-  __shared__ float most_of[kAppendThreads / 64];
+  constexpr int VEC = 16 / E::kBytes;
+  constexpr int LPT = D / VEC;  // 8 .. 64
+  constexpr int TPI = 64 / LPT;
+  using P = Pack<S, VEC>;
+  const uint32_t tile = blockIdx.x / static_cast<uint32_t>(a.unit_blocks);
   PageTile t;
-  if (!page_tile(a, static_cast<int>(blockIdx.x), &t)) return;
-  const int h = blockIdx.y, which = blockIdx.z;
-  const S* x = static_cast<const S*>(a.x[which]) + t.row * a.token_stride[which] + h * a.head_stride[which];
-  const int64_t row_bytes = static_cast<int64_t>(a.heads) * a.dim;
-  uint8_t* codes = a.cache[which] + t.phys * a.page * row_bytes + static_cast<int64_t>(h) * a.dim;
-  const int n = (t.t1 - t.t0) * a.dim;
-  auto x_of = [&](int i) { return E::to_f32(x[(i / a.dim) * a.token_stride[which] + i % a.dim]); };
-  float most = 0.0f;
-  for (int i = threadIdx.x; i < n; i += kAppendThreads) most = fmaxf(most, finite_abs(x_of(i)));
-  most = wave_max(most);
-  if (__lane_id() == 0) most_of[threadIdx.x >> 6] = most;
-  float* scale_at = a.scale[which] + t.phys * a.heads + h;
-  const float old = *scale_at;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kAppendThreads / 64; ++w) most = fmaxf(most, most_of[w]);
+  if (!page_tile(a, static_cast<int>(tile), &t)) return;
+  const int lane = __lane_id();
+  const int tok = lane / LPT, dim = VEC * (lane % LPT);
+  const int n = t.t1 - t.t0;
+  const int packs = (n + TPI - 1) / TPI;
+  const bool once = packs <= HOLD;
   const bool held = t.t0 > 0;
+  const int unit = static_cast<int>(blockIdx.x - tile * a.unit_blocks) * kAppendWaves + wave_id();
+  if (unit >= 2 * a.heads) return;
+  const int which = unit & 1, h = unit >> 1;
+  const int64_t x_row = which ? a.token_stride[1] : a.token_stride[0];
+  const S* x = static_cast<const S*>(which ? a.x[1] : a.x[0]) + t.row * x_row +
+               h * (which ? a.head_stride[1] : a.head_stride[0]) + dim;
+  // Pack i of the tile; a lane past the last token reads that again, which changes
+  // neither the largest magnitude nor the bounds.
+  auto load = [&](int i) {
+    const S* p = x + min(i * TPI + tok, n - 1) * x_row;
+    if constexpr (ALIGNED) {
+      return __builtin_bit_cast(P, global_load16_nt(reinterpret_cast<const char*>(p)));
+    } else {
+      return load_at<false, P>(p, 0);
+    }
+  };
+  P v[HOLD] = {};
+  auto load_all = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      if (base + i < packs) v[i] = load(base + i);
+    }
+  };
+  load_all(0);  // on its way while the page's entry arrives
+  if (t.phys < 0 || t.phys >= a.num_pages) return;
+
+  const int64_t row_bytes = static_cast<int64_t>(a.heads) * D;
+  const int64_t head = static_cast<int64_t>(t.phys) * a.heads + h;
+  uint8_t* codes = (which ? a.cache[1] : a.cache[0]) + t.phys * (a.page * row_bytes) + static_cast<int64_t>(h) * D;
+  float* scale_at = (which ? a.scale[1] : a.scale[0]) + head;
+  const bool bounded = which == 0 && a.bounds != nullptr;
+  // The page's bounds, D smallest then D largest codes: this lane's `words` of four
+  // (see the end), its sign +1 for smallest and -1 for largest.
+  constexpr int SETS = LPT == 64 ? 2 : 1;
+  constexpr int WORDS = LPT == 32 ? VEC / 4 : 1;  // of a set
+  const bool upper = LPT < 64 && lane >= 32;
+  uint32_t* edge = nullptr;
+  bool edge_lane = false;
+  if (bounded) {
+    edge = reinterpret_cast<uint32_t*>(a.bounds + head * 2 * D + (upper ? D : 0) + dim +
+                                       (VEC == 8 && LPT <= 16 ? 4 * ((lane >> 4) & 1) : 0));
+    edge_lane = !(LPT == 16 && VEC == 4 && (lane & 16) != 0) && !(LPT == 8 && (lane & 8) != 0);
+  }
+  // What the page has.
+  float old = 0.0f;
+  uint32_t held_edge[SETS][WORDS] = {};
+  if (held) {
+    old = *scale_at;
+    if (edge_lane) {
+#pragma unroll
+      for (int s = 0; s < SETS; ++s) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) held_edge[s][i] = edge[s * (D / 4) + i];
+      }
+    }
+  }
+
+  // Largest magnitude of the finite values, or, in each dimension, their smallest
+  // (end[0]) and the smallest of their negatives (end[1]).
+  float end[2][VEC];
+  float most = 0.0f;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) end[0][j] = end[1][j] = INFINITY;
+  auto scan = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      if (base + i < packs) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float f = finite_or_nan(E::to_f32(v[i].v[j]));
+          if (bounded) {
+            end[0][j] = fminf(end[0][j], f);
+            end[1][j] = fminf(end[1][j], -f);
+          } else {
+            most = fmaxf(most, fabsf(f));
+          }
+        }
+      }
+    }
+  };
+  scan(0);
+  for (int base = HOLD; base < packs; base += HOLD) {
+    load_all(base);
+    scan(base);
+  }
+  if (bounded) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) most = fmaxf(most, fmaxf(finite_abs(end[0][j]), finite_abs(end[1][j])));
+  }
+  most = max_xor32(max_xor16(row16_max(most)));
+  // The packs stay packed until here: widened once for both their scan and their
+  // codes (the compiler's choice otherwise) they would take twice the registers.
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i) {
+    u32x4 r = __builtin_bit_cast(u32x4, v[i]);
+    asm volatile("" : "+v"(r));
+    v[i] = __builtin_bit_cast(P, r);
+  }
+
   const float fresh = e4m3_scale(most);
   const float scale = held ? fmaxf(old, fresh) : fresh;
-  const bool grown = held && scale > old;
-  if (threadIdx.x == 0) *scale_at = scale;
-  auto again = [&](uint8_t c) { return e4m3((e4m3_value(c) * old) / scale); };
+  const bool grown = __builtin_amdgcn_readfirstlane(held && scale > old);
+  if (lane == 0) *scale_at = scale;
+  const Over over(scale);
+  // A held code's value, over the page's new scale.
+  auto again = [&](float value) { return over(value * old); };
   if (grown) {
-    for (int i = threadIdx.x; i < t.t0 * a.dim; i += kAppendThreads) {
-      uint8_t* c = codes + (i / a.dim) * row_bytes + i % a.dim;
-      *c = again(*c);
+    constexpr int kLanes = D / 16;
+    for (int s = lane / kLanes; s < t.t0; s += 64 / kLanes) {
+      u32x4* c = reinterpret_cast<u32x4*>(codes + s * row_bytes + 16 * (lane % kLanes));
+      const u32x4 w = *c;
+      u32x4 r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        r[i] = e4m3x4(again(e4m3_value_at<0>(w[i])), again(e4m3_value_at<1>(w[i])), again(e4m3_value_at<2>(w[i])),
+                      again(e4m3_value_at<3>(w[i])));
+      }
+      *c = r;
     }
   }
-  for (int i = threadIdx.x; i < n; i += kAppendThreads) {
-    codes[(t.t0 + i / a.dim) * row_bytes + i % a.dim] = e4m3(x_of(i) / scale);
+  auto write = [&](int i, const P& p) {
+    const int s = i * TPI + tok;
+    if (s >= n) return;
+    float c[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) c[j] = over(E::to_f32(p.v[j]));
+    store_codes<true>(codes + (t.t0 + s) * row_bytes, dim, c);
+  };
+  if (once) {
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      if (i < packs) write(i, v[i]);
+    }
+  } else {
+    for (int i = 0; i < packs; ++i) write(i, load(i));
   }
-  if (which == 0 && a.bounds != nullptr) {
-    uint8_t* edge = a.bounds + (t.phys * a.heads + h) * 2 * a.dim;
-    for (int d = threadIdx.x; d < a.dim; d += kAppendThreads) {
-      // NaN codes take no part.
-      float lo = kE4M3Max, hi = -kE4M3Max;
-      if (held) {
-        lo = fminf(lo, e4m3_value(grown ? again(edge[d]) : edge[d]));
-        hi = fmaxf(hi, e4m3_value(grown ? again(edge[a.dim + d]) : edge[a.dim + d]));
-      }
-      for (int i = 0; i < t.t1 - t.t0; ++i) {
-        const float c = e4m3_value(e4m3(x_of(i * a.dim + d) / scale));
-        lo = fminf(lo, c);
-        hi = fmaxf(hi, c);
-      }
-      edge[d] = e4m3(lo);
-      edge[a.dim + d] = e4m3(hi);
+
+  if (!bounded) return;
+  // The lanes that hold other tokens' values of the same dimensions give theirs up
+  // by halves: lanes below 32 keep the smallest and those above the largest, then,
+  // of 16-bit types, even rows of 16 the first four dimensions and odd rows the last
+  // four. A division by the scale and the rounding to a code are both monotone, so
+  // the bounds of the codes are the codes of the bounds, and a held bound may join
+  // before they are rounded. A dimension without a finite value keeps +448 and -448.
+  float mine[SETS][VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    if constexpr (SETS == 2) {
+      mine[0][j] = end[0][j];
+      mine[1][j] = end[1][j];
+    } else {
+      mine[0][j] = min_swap32(end[0][j], end[1][j]);
     }
   }
+  if constexpr (LPT <= 16) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mine[0][j] = min_swap16(mine[0][j], mine[0][VEC == 8 ? j + 4 : j]);
+  }
+  if constexpr (LPT <= 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mine[0][j] = fminf(mine[0][j], dpp<kDppRowRor8>(mine[0][j]));
+  }
+  if (!edge_lane) return;
+#pragma unroll
+  for (int s = 0; s < SETS; ++s) {
+    const float sign = upper || s == 1 ? -1.0f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      float c[4];
+      const uint32_t w = held_edge[s][i];
+      const float was[4] = {e4m3_value_at<0>(w), e4m3_value_at<1>(w), e4m3_value_at<2>(w), e4m3_value_at<3>(w)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float m = mine[s][4 * i + j];
+        c[j] = m < INFINITY ? over(m) : kE4M3Max;
+        if (held) c[j] = fminf(c[j], sign * (grown ? again(was[j]) : was[j]));
+        c[j] *= sign;
+      }
+      edge[s * (D / 4) + i] = e4m3x4(c[0], c[1], c[2], c[3]);
+    }
+  }
+}
+
+// Calls f(IntC<D>, IntC<HOLD>) for the kernel that serves the head size, pages of
+// `packs` packs a lane, and single tokens or chunks.
+template <int N>
+using IntC = std::integral_constant<int, N>;
+template <typename F>
+void dispatch_append(int dim, int packs, bool chunks, F&& f) {
+  auto with_dim = [&](auto d) {
+    if (!chunks) {
+      f(d, IntC<1>{});
+    } else if (packs <= 4) {
+      f(d, IntC<4>{});
+    } else {
+      f(d, IntC<16>{});
+    }
+  };
+  if (dim == 64) {
+    with_dim(IntC<64>{});
+  } else if (dim == 128) {
+    with_dim(IntC<128>{});
+  } else {
+    with_dim(IntC<256>{});
+  }
+}
+
+template <typename E>
+int launch_append(AppendArgs& a, int64_t tiles, hipStream_t stream) {
+  auto aligned = [&](int i) {
+    return reinterpret_cast<uintptr_t>(a.x[i]) % 16 == 0 && a.token_stride[i] * E::kBytes % 16 == 0 &&
+           a.head_stride[i] * E::kBytes % 16 == 0;
+  };
+  const bool al = aligned(0) && aligned(1);
+  const int packs = static_cast<int>(cdiv(static_cast<int64_t>(a.page) * a.dim * E::kBytes, 1024));
+  int st = KL_OK;
+  dispatch_append(a.dim, packs, a.offsets != nullptr, [&](auto d, auto hold) {
+    constexpr int D = decltype(d)::value, HOLD = decltype(hold)::value;
+    const int64_t wgs = cdiv(2 * static_cast<int64_t>(a.heads), kAppendWaves);
+    if (tiles * wgs > 0xffffffffLL / kAppendThreads) {
+      st = fail(KL_ERR_UNSUPPORTED, "too many tokens, sequences or heads for one launch");
+      return;
+    }
+    a.unit_blocks = static_cast<int>(wgs);
+    const auto grid = static_cast<unsigned>(tiles * wgs);
+    if (al) {
+      append_kernel<E, D, HOLD, true><<<grid, kAppendThreads, 0, stream>>>(a);
+    } else {
+      append_kernel<E, D, HOLD, false><<<grid, kAppendThreads, 0, stream>>>(a);
+    }
+  });
+  return st != KL_OK ? st : check_launch("append_kv_fp8 kernel launch");
 }
 
 // -------------------------------------------------------------------- select
@@ -301,9 +540,6 @@ extern "C" int kl_append_kv_fp8(kl_dtype dtype, void* k_cache, void* v_cache, fl
   if (batch < 0 || tokens < 0 || num_kv_heads <= 0 || head_dim <= 0 || page_size <= 0 || num_pages < 0 || max_pages < 0) {
     return fail(KL_ERR_INVALID_ARGUMENT, "tokens, batch, heads, head_dim, page_size, num_pages and max_pages must be positive");
   }
-  if (dtype != KL_DTYPE_F32 && dtype != KL_DTYPE_F16 && dtype != KL_DTYPE_BF16) {
-    return fail(KL_ERR_UNSUPPORTED, "dtype must be f32, f16 or bf16");
-  }
   if (!head_dim_ok(head_dim) || page_size % 16 != 0) {
     return fail(KL_ERR_UNSUPPORTED, "an FP8 cache needs head_dim 64, 128 or 256 and page_size a multiple of 16");
   }
@@ -317,8 +553,12 @@ extern "C" int kl_append_kv_fp8(kl_dtype dtype, void* k_cache, void* v_cache, fl
   if (block_table_stride < max_pages && batch > 1) {
     return fail(KL_ERR_INVALID_ARGUMENT, "block_table_stride must be >= max_pages");
   }
+  if (reinterpret_cast<uintptr_t>(k_cache) % 16 != 0 || reinterpret_cast<uintptr_t>(v_cache) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(k_bounds) % 16 != 0) {
+    return fail(KL_ERR_INVALID_ARGUMENT, "the caches and k_bounds must be 16-byte aligned");
+  }
   const int64_t tiles = new_offsets == nullptr ? batch : tokens / page_size + 2 * static_cast<int64_t>(batch);
-  if (tokens > 0x7fffffffLL || tiles > 0x7fffffffLL / kAppendThreads || num_kv_heads > 65535) {
+  if (tokens > 0x7fffffffLL || tiles > 0x7fffffffLL) {
     return fail(KL_ERR_UNSUPPORTED, "too many tokens, sequences or heads for one launch");
   }
   AppendArgs a;
@@ -344,20 +584,16 @@ extern "C" int kl_append_kv_fp8(kl_dtype dtype, void* k_cache, void* v_cache, fl
   a.page = page_size;
   a.max_pages = max_pages;
   a.num_pages = num_pages;
-  const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(num_kv_heads), 2);
   const auto s = reinterpret_cast<hipStream_t>(stream);
   switch (dtype) {
     case KL_DTYPE_F32:
-      append_kernel<F32><<<grid, kAppendThreads, 0, s>>>(a);
-      break;
+      return launch_append<F32>(a, tiles, s);
     case KL_DTYPE_F16:
-      append_kernel<F16><<<grid, kAppendThreads, 0, s>>>(a);
-      break;
+      return launch_append<F16>(a, tiles, s);
     case KL_DTYPE_BF16:
-      append_kernel<BF16><<<grid, kAppendThreads, 0, s>>>(a);
-      break;
+      return launch_append<BF16>(a, tiles, s);
   }
-  return check_launch("append_kv_fp8 kernel launch");
+  return fail(KL_ERR_UNSUPPORTED, "dtype must be f32, f16 or bf16");
 }
 
 extern "C" int kl_select_pages_workspace(int batch, int num_kv_heads, int max_pages, size_t* out_workspace) {
