@@ -391,9 +391,20 @@ int launch_append(AppendArgs& a, int64_t tiles, hipStream_t stream) {
 // The largest q.k that a key within the page's bounds can have, for the query
 // head of the KV head's group where it is largest:
 //   score = f32(k_scale * max_g sum_d max(q_gd lo_d, q_gd hi_d))
-// The sum is formed in 64 bits, where it is exact for queries whose values span
-// less than about 2^30 (a product has 15 bits at most), so the order of its
-// terms does not decide which of two near scores is larger.
+//         = f32(k_scale * max_g [lo hi] . [min(q_g, 0) max(q_g, 0)])
+// The sum is one of 64 bits, where it is exact for queries whose values span less
+// than about 2^30 (a product has 15 bits at most), so the order of its terms does
+// not decide which of two near scores is larger. In 64 bits for every page, the
+// scores took 25 us of 8 x 1,024 pages on 8 CUs even on the fp64 matrix cores; so:
+//   1. scores of all pages on the 16-bit matrix cores, summed in fp32 and within
+//      kScoreSlack of their own size;
+//   2. the bin of a histogram over them that holds the smallest such score kept, T. The
+//      smallest true score kept is within E, the largest error of a page, of it, so
+//      pages more than 2 E above the bin are kept and those more than 2 E below it are
+//      not, whatever their sums in 64 bits are;
+//   3. scores in 64 bits for the pages between (some ten of a thousand), and the choice
+//      among them.
+// Where a score is not finite, every page is one between.
 struct SelectArgs {
   const void* q;
   const uint8_t* bounds;
@@ -401,128 +412,511 @@ struct SelectArgs {
   const int32_t* table;
   const int32_t* seq_lens;
   int64_t bt_stride;
-  float* scores;  // [batch, kv heads, max_pages]
+  uint32_t* keys;  // [batch, kv heads, max_pages], where the scores have a launch of their own
   int32_t* out_table;
   int32_t* out_lens;
-  int batch, heads, group, dim, page, max_pages, keep, first, last;
+  int batch, heads, group, page, max_pages, keep, first, last;
 };
 
 __device__ __forceinline__ int select_len(const SelectArgs& a, int b) {
   const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page;
-  const int64_t len = a.seq_lens[b];
+  const int64_t len = as_constant(a.seq_lens)[b];
   return static_cast<int>(max(static_cast<int64_t>(0), min(len, cap)));
 }
 
-// A page's score as a key that orders like it: pinned pages before all others, a
-// NaN like the largest finite score.
+// A score as a key that orders like it; a NaN like the largest finite score.
 __device__ __forceinline__ uint32_t score_key(float s) {
   s = s < 0x1.fffffep127f ? s : 0x1.fffffep127f;
   const uint32_t u = __builtin_bit_cast(uint32_t, s == 0.0f ? 0.0f : s);
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// A wave per page.
+// The score of a key made from a finite one.
+__device__ __forceinline__ float key_score(uint32_t key) {
+  return __builtin_bit_cast(float, (key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+
+// Keys beside those of finite scores: certainly kept (step 3), and a score that is
+// not finite (step 1).
+constexpr uint32_t kKeyKept = 0xfffffffeu, kKeyNotFinite = 0xffffffffu;
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = dpp_u32<CTRL>(static_cast<uint32_t>(u)), hi = dpp_u32<CTRL>(static_cast<uint32_t>(u >> 32));
+  return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+}
+
+// The larger of two, NaN if either is.
+__device__ __forceinline__ double max_or_nan(double a, double b) { return a != a || a > b ? a : b; }
+
+// 16-bit matrix products: 16 pages by 16 query heads, 32 bytes of the bounds a step.
+// Lane l supplies A[page l % 16] and B[head l % 16] for eight k of group l / 16 and gets
+// the scores of pages 4 (l / 16) .. + 3 and head l % 16. Which bytes a step's k are is
+// free as long as A and B agree: a lane's load of 16 codes is its eight k of two steps.
 template <typename E>
-__global__ void __launch_bounds__(256) score_kernel(const SelectArgs a) {
-  const int64_t unit = blockIdx.y;
-  const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
-  const int pages = (select_len(a, b) + a.page - 1) / a.page;
-  const int p = blockIdx.x * 4 + wave_id();
-  if (p >= pages) return;
-  const int64_t phys = a.table[b * a.bt_stride + p];
-  const uint8_t* edge = a.bounds + (phys * a.heads + h) * 2 * a.dim;
-  const typename E::S* q = static_cast<const typename E::S*>(a.q) + unit * a.group * a.dim;
-  double best = -INFINITY;
-  for (int g = 0; g < a.group; ++g) {
-    double sum = 0.0;
-    for (int d = __lane_id(); d < a.dim; d += 64) {
-      const float qv = E::to_f32(q[g * a.dim + d]);
-      sum += static_cast<double>(qv) * static_cast<double>(e4m3_value(qv < 0.0f ? edge[d] : edge[a.dim + d]));
-    }
-    for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
-    best = sum > best || sum != sum ? sum : best;
-  }
-  if (__lane_id() == 0) {
-    a.scores[unit * a.max_pages + p] = static_cast<float>(best * static_cast<double>(a.scale[phys * a.heads + h]));
+__device__ __forceinline__ f32x4 score_mma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (std::is_same_v<E, F16>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
 }
 
-constexpr int kPickThreads = 256;
+constexpr int kHeadsAtOnce = 16;
 
-// A workgroup per (sequence, KV head): the keep-th largest key by four passes of
-// eight bits over a histogram, then the pages above it, and as many of its equals
-// as are wanted, lowest first, in ascending order.
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) {
-  __shared__ int hist[256];
-  __shared__ int wave_count[2][kPickThreads / 64];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_want;
-  const int64_t unit = blockIdx.x;
-  const int b = static_cast<int>(unit / a.heads);
-  const int len = select_len(a, b);
-  const int pages = (len + a.page - 1) / a.page;
-  const int kept = min(pages, a.keep);
-  const float* scores = a.scores + unit * a.max_pages;
+// Query heads g0 .. g0 + 15 of a unit as the B operands, heads past the group as zeros:
+// lane l's eight values of step 2 c + half are byte 64 c + 16 (l / 16) + 8 half of
+// [lo hi] on, so min(q, 0) in the first half of the steps and max(q, 0) in the others.
+template <typename E, int D>
+struct ScoreQueries {
+  static constexpr int C = 2 * D / 64;
+  u32x4 v[C][2];
+  __device__ __forceinline__ ScoreQueries(const SelectArgs& a, int64_t unit, int g0) {
+    const int lane = __lane_id(), g = g0 + (lane & 15);
+    const auto* q = static_cast<const typename E::S*>(a.q) + (unit * a.group + min(g, a.group - 1)) * D + 16 * (lane >> 4);
+#pragma unroll
+    for (int c = 0; c < C / 2; ++c) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const u32x4 w = g < a.group ? *reinterpret_cast<const u32x4*>(q + 64 * c + 8 * half) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // 0xffff in the halves that are negative (a NaN of either sign reaches one side).
+          const uint32_t sign = (w[i] >> 15) & 0x00010001u;
+          const uint32_t negative = (sign << 16) - sign;
+          v[c][half][i] = w[i] & negative;
+          v[c + C / 2][half][i] = w[i] & ~negative;
+        }
+      }
+    }
+  }
+};
+
+// The keys, from step 1's scores, of pages 16 tile .. 16 tile + 15 of a unit, by a
+// wave: store(page, key). Returns the largest k_scale that the lane has seen.
+template <typename E, int D, typename Store>
+__device__ __forceinline__ float score_tile(const SelectArgs& a, const ScoreQueries<E, D>& q, int b, int h, int g0,
+                                            int pages, int tile, Store&& store) {
+  constexpr int C = 2 * D / 64;
+  const int lane = __lane_id(), k = lane >> 4;
+  const int32_t* table = a.table + b * a.bt_stride;
+  const int phys = table[min(16 * tile + (lane & 15), pages - 1)];
+  const int64_t head = static_cast<int64_t>(phys) * a.heads + h;
+  const uint8_t* edge = a.bounds + head * (2 * D) + 16 * k;
+  u32x4 w[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) w[c] = *reinterpret_cast<const u32x4*>(edge + 64 * c);
+  const float scale = a.scale[head];
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    u32x4 lo, hi;
+    fp8x16_to<E>(w[c], lo, hi);
+    s = score_mma<E>(lo, q.v[c][0], s);
+    s = score_mma<E>(hi, q.v[c][1], s);
+  }
+  // Lane 4 k + i of the 16 gets page 4 k + i's score; a maximum drops a NaN, a sum keeps it.
+  const bool valid = g0 + (lane & 15) < a.group;
+  float mine = 0.0f, check = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float m = row16_max(valid ? s[i] : -INFINITY), n = row16_sum(valid ? s[i] * 0.0f : 0.0f);
+    if ((lane & 3) == i) {
+      mine = m;
+      check = n;
+    }
+  }
+  const int m = 4 * k + (lane & 3);
+  const float m_scale = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * m, __builtin_bit_cast(int, scale)));
+  const float score = mine * m_scale + check;
+  const int page = 16 * tile + m;
+  if ((lane & 15) < 4 && page < pages) store(page, fabsf(score) < INFINITY ? score_key(score) : kKeyNotFinite);
+  return scale;
+}
+
+// Keys of tiles first, first + step, ... of a unit into keys[page], by a wave. Groups of
+// more than kHeadsAtOnce heads take several rounds: a scale is not negative, so the
+// maximum over heads may be taken after the product with it.
+template <typename E, int D>
+__device__ __forceinline__ float score_unit(const SelectArgs& a, int64_t unit, int b, int h, int pages, int first,
+                                            int step, uint32_t* keys) {
+  const int tiles = (pages + 15) / 16;
+  float most = 0.0f;
+  for (int g0 = 0; g0 < a.group; g0 += kHeadsAtOnce) {
+    const ScoreQueries<E, D> q(a, unit, g0);
+    for (int tile = first; tile < tiles; tile += step) {
+      most = fmaxf(most, score_tile<E, D>(a, q, b, h, g0, pages, tile, [&](int page, uint32_t key) {
+                     keys[page] = g0 == 0 ? key : max(keys[page], key);
+                   }));
+    }
+  }
+  return most;
+}
+
+// How far step 1's score may be from the true one, over the sum of its terms' sizes: a
+// sum of head_dim products (the others are zeros), head_dim <= 256, takes at most 256
+// roundings of 2^-23 each (or truncations), 2^-15; twice that.
+constexpr float kScoreSlack = 0x1p-14f;
+
+// max_g sum_d |q_gd| over a unit's heads g = first, first + step, ..., by a wave.
+template <typename E, int D>
+__device__ __forceinline__ float query_size(const SelectArgs& a, int64_t unit, int first, int step) {
+  const auto* q = static_cast<const typename E::S*>(a.q) + unit * a.group * D;
+  float most = 0.0f;
+  for (int g = first; g < a.group; g += step) {
+    float sum = 0.0f;
+    for (int d = __lane_id(); d < D; d += 64) sum += fabsf(E::to_f32(q[g * D + d]));
+    most = fmaxf(most, wave_sum(sum));
+  }
+  return most;
+}
+
+// The true score's key of a page, by a wave: each row of 16 lanes a query head, each
+// lane D / 16 dimensions.
+template <typename E, int D>
+__device__ __forceinline__ uint32_t true_key(const SelectArgs& a, int64_t unit, int b, int h, int page) {
+  constexpr int N = D / 16;
+  const int lane = __lane_id(), d0 = N * (lane & 15);
+  const int64_t head = static_cast<int64_t>(a.table[b * a.bt_stride + page]) * a.heads + h;
+  const uint8_t* edge = a.bounds + head * (2 * D) + d0;
+  const double scale = a.scale[head];
+  double best = -INFINITY;
+  for (int g0 = 0; g0 < a.group; g0 += 4) {
+    const int g = g0 + (lane >> 4);
+    const auto* q = static_cast<const typename E::S*>(a.q) + (unit * a.group + min(g, a.group - 1)) * D + d0;
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float v = E::to_f32(q[i]);
+      sum = fma(static_cast<double>(v < 0.0f ? v : 0.0f), static_cast<double>(e4m3_value(edge[i])), sum);
+      sum = fma(static_cast<double>(v < 0.0f ? 0.0f : v), static_cast<double>(e4m3_value(edge[D + i])), sum);
+    }
+    sum += dpp64<kDppQuadSwap1>(sum);
+    sum += dpp64<kDppQuadSwap2>(sum);
+    sum += dpp64<kDppRowRor4>(sum);
+    sum += dpp64<kDppRowRor8>(sum);
+    if (g < a.group) best = max_or_nan(sum, best);
+  }
+  for (int m = 16; m <= 32; m *= 2) best = max_or_nan(best, __shfl_xor(best, m));
+  return score_key(static_cast<float>(best * scale));
+}
+
+constexpr int kScoreWaves = 4;
+
+// Step 1 in a launch of its own: workgroups along x share a unit's tiles.
+template <typename E, int D>
+__global__ void __launch_bounds__(kScoreWaves * 64) score_kernel(const SelectArgs a) {
+  const int64_t unit = blockIdx.y;
+  const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
+  const int pages = (select_len(a, b) + a.page - 1) / a.page;
+  const int first = static_cast<int>(blockIdx.x) * kScoreWaves + wave_id();
+  if (16 * first >= pages || pages <= a.keep) return;
+  score_unit<E, D>(a, unit, b, h, pages, first, kScoreWaves * static_cast<int>(gridDim.x), a.keys + unit * a.max_pages);
+}
+
+constexpr int kPickWaves = 16;
+constexpr int kPickThreads = kPickWaves * 64;
+
+constexpr int kBins = kPickThreads;
+constexpr int kListed = 64;  // pages between that a wave ranks
+
+struct PickLds {
+  int count[2][3][kPickWaves];  // of two rounds in turn, so that a round needs one barrier
+  float scale[kPickWaves], size[kPickWaves];
+  uint32_t low[kPickWaves], high[kPickWaves];
+  int bins[kBins];
+  int bin;                    // that holds T
+  int kept, between;          // pages certainly kept, pages between
+  int list[kListed];          // the first of them, and their keys
+  uint32_t list_key[kListed];
+};
+
+// Before the first barrier of pick_pages.
+__device__ __forceinline__ void clear(PickLds& lds) {
+  lds.bins[threadIdx.x] = 0;
+  if (threadIdx.x == 0) lds.kept = lds.between = 0;
+}
+
+// The smallest of the `want` largest keys of pages [q0, q1) of all threads, by a
+// workgroup of kPickThreads.
+//
+// The interval that holds it is cut in four: each round counts the keys from three
+// thresholds on. It ends as soon as a threshold leaves exactly the number wanted, after
+// about half of log2(pages) rounds beyond the bits that all keys share; only equal keys
+// take it to the end. For selections that have many pages between (equal or nearly
+// equal scores): a round's counts go through LDS, and 15 of them took 20 us.
+template <typename Key>
+__device__ uint32_t smallest_kept(PickLds& lds, int want, int q0, int q1, uint32_t low, uint32_t high, Key&& key) {
+  const int wave = wave_id(), lane = __lane_id();
+  // Keys from `low` on are `want` at least, from high + 1 on fewer.
+  for (int round = 0; low < high; ++round) {
+    const uint32_t step = (high - low) / 4;
+    const uint32_t t[3] = {low + step + 1, low + 2 * step + 1, low + 3 * step + 1};
+    int n[3] = {0, 0, 0};
+    for (int p = q0; p < q1; ++p) {
+      const uint32_t k = key(p);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) n[i] += k >= t[i] ? 1 : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int total = __builtin_amdgcn_readlane(wave_prefix_sum(n[i]), 63);
+      if (lane == 0) lds.count[round & 1][i][wave] = total;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      n[i] = 0;
+      for (int w = 0; w < kPickWaves; ++w) n[i] += lds.count[round & 1][i][w];
+    }
+    const int side = n[2] >= want ? 3 : n[1] >= want ? 2 : n[0] >= want ? 1 : 0;
+    if (side < 3) high = t[side] - 1;
+    if (side > 0) {
+      low = t[side - 1];
+      if (n[side - 1] == want) break;  // the keys from low on are the ones kept
+    }
+  }
+  __syncthreads();  // before the counts' next use
+  return low;
+}
+
+// Steps 2 and 3, by a workgroup of kPickThreads: a unit's pages from its keys. scale: the
+// largest k_scale that the lane has seen of the unit's pages.
+template <typename E, int D>
+__device__ void pick_pages(const SelectArgs& a, PickLds& lds, int64_t unit, int b, int h, int pages, uint32_t* keys,
+                           float scale) {
+  const int wave = wave_id(), lane = __lane_id();
+  const int kept = a.keep;  // < pages
   const int32_t* table = a.table + b * a.bt_stride;
   int32_t* out = a.out_table + unit * a.keep;
-  for (int i = kept + threadIdx.x; i < a.keep; i += kPickThreads) out[i] = 0;
+  // A thread's pages are neighbours, so that ranks in the sequence are prefix sums.
+  const int each = (pages + kPickThreads - 1) / kPickThreads;
+  const int p0 = min(static_cast<int>(threadIdx.x) * each, pages), p1 = min(p0 + each, pages);
+  const int free0 = a.first, free1 = pages - a.last;  // pages that are not pinned
+  const int q0 = max(p0, free0), q1 = min(p1, free1);
+  const int want = kept - a.first - a.last;
+  auto key = [&](int p) { return keys[p]; };
+
+  scale = max_xor32(max_xor16(row16_max(scale)));
+  const float size = query_size<E, D>(a, unit, wave, kPickWaves);
+  if (lane == 0) {
+    lds.scale[wave] = scale;
+    lds.size[wave] = size;
+  }
+  __syncthreads();  // the keys are there, too
+  uint32_t low = 0xffffffffu, high = 0;
+  for (int p = q0; p < q1; ++p) {
+    low = min(low, key(p));
+    high = max(high, key(p));
+  }
+  for (int m = 32; m > 0; m >>= 1) {
+    low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), m)));
+    high = max(high, static_cast<uint32_t>(__shfl_xor(static_cast<int>(high), m)));
+  }
+  if (lane == 0) {
+    lds.low[wave] = low;
+    lds.high[wave] = high;
+  }
+  __syncthreads();
+  low = lds.low[lane % kPickWaves];
+  high = lds.high[lane % kPickWaves];
+  scale = row16_max(lds.scale[lane % kPickWaves]);
+  const float most_size = row16_max(lds.size[lane % kPickWaves]);
+  for (int m = 8; m > 0; m >>= 1) {
+    low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), m)));
+    high = max(high, static_cast<uint32_t>(__shfl_xor(static_cast<int>(high), m)));
+  }
+  uint32_t least = 0xffffffffu;  // the smallest key kept: none but the pinned pages
+  if (want > 0) {
+    // Step 2. What underflows in 16 bits adds less than the last term.
+    const float reach = 2.0f * (kScoreSlack * kE4M3Max * most_size * scale) + 0x1p-100f;
+    const float lowest = key_score(low), width = key_score(high) - lowest;
+    const bool finite = high != kKeyNotFinite && reach < INFINITY && width < INFINITY;
+    // Monotone, so a score of a higher bin is a higher one.
+    const float to_bin = width > 0.0f ? fminf(kBins / width, 0x1p100f) : 0.0f;
+    auto bin_of = [&](float s) { return static_cast<int>(fminf(fmaxf((s - lowest) * to_bin, -1.0f), 1.0f * kBins)); };
+    int bin = 0;
+    if (finite) {
+      for (int p = q0; p < q1; ++p) atomicAdd(&lds.bins[min(bin_of(key_score(key(p))), kBins - 1)], 1);
+      __syncthreads();
+      // Thread t has bin kBins - 1 - t; the pages from it upwards.
+      const int mine = lds.bins[kBins - 1 - static_cast<int>(threadIdx.x)];
+      int upto = wave_prefix_sum(mine);
+      if (lane == 63) lds.count[0][0][wave] = upto;
+      __syncthreads();
+      const int ahead = lane < wave ? lds.count[0][0][lane % kPickWaves] : 0;
+      upto += __builtin_amdgcn_readlane(wave_prefix_sum(ahead), 63);
+      if (upto >= want && upto - mine < want) lds.bin = kBins - 1 - static_cast<int>(threadIdx.x);
+      __syncthreads();
+      bin = lds.bin;
+    }
+    // Step 3. The pages between are listed in the order that they come in; which of them
+    // are kept does not depend on it. (The last bin takes what is past its end, too.)
+    for (int p = q0; p < q1; ++p) {
+      const float s = key_score(key(p));
+      if (finite && bin < kBins - 1 && bin_of(s - reach) > bin) {
+        keys[p] = kKeyKept;
+        atomicAdd(&lds.kept, 1);
+      } else if (finite && bin_of(s + reach) < bin) {
+        keys[p] = 0;
+      } else {
+        keys[p] = kKeyNotFinite;  // to be scored
+        const int i = atomicAdd(&lds.between, 1);
+        if (i < kListed) lds.list[i] = p;
+      }
+    }
+    __syncthreads();
+    const int between = lds.between;
+    if (between <= kListed) {
+      for (int i = wave; i < between; i += kPickWaves) {
+        const uint32_t k = true_key<E, D>(a, unit, b, h, __builtin_amdgcn_readfirstlane(lds.list[i]));
+        if (lane == 0) lds.list_key[i] = k;
+      }
+      __syncthreads();
+      if (wave == 0) {
+        const bool mine = lane < between;
+        const int p = mine ? lds.list[lane] : 0;
+        const uint32_t k = mine ? lds.list_key[lane] : 0;
+        int better = 0;
+        for (int i = 0; i < between; ++i) {
+          const uint32_t ki = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k), i));
+          const int pi = __builtin_amdgcn_readlane(p, i);
+          better += ki > k || (ki == k && pi < p) ? 1 : 0;
+        }
+        if (mine) keys[p] = better < want - lds.kept ? kKeyKept : 0;
+      }
+      __syncthreads();
+      least = kKeyKept;
+    } else {
+      for (int base = wave * 64; base < pages; base += kPickThreads) {
+        const int p = base + lane;
+        uint64_t todo = __ballot(p >= free0 && p < free1 && keys[min(p, pages - 1)] == kKeyNotFinite);
+        for (; todo != 0; todo &= todo - 1) {
+          const int at = base + __builtin_ctzll(todo);
+          const uint32_t k = true_key<E, D>(a, unit, b, h, at);
+          if (lane == 0) keys[at] = k;
+        }
+      }
+      __syncthreads();
+      least = smallest_kept(lds, want, q0, q1, 0, kKeyKept, key);
+    }
+  }
+
+  // Positions: pages above the smallest key kept, and the first ones equal to it.
+  int above = max(0, min(p1, free0) - p0) + max(0, p1 - max(p0, free1)), ties = 0;
+  for (int p = q0; p < q1; ++p) {
+    const uint32_t k = key(p);
+    above += k > least ? 1 : 0;
+    ties += k == least ? 1 : 0;
+  }
+  const int above_to = wave_prefix_sum(above), ties_to = wave_prefix_sum(ties);
+  if (lane == 63) {
+    lds.count[1][0][wave] = above_to;
+    lds.count[1][1][wave] = ties_to;
+  }
+  __syncthreads();
+  const int above_before = wave_prefix_sum(lane < kPickWaves ? lds.count[1][0][lane % kPickWaves] : 0);
+  const int ties_before = wave_prefix_sum(lane < kPickWaves ? lds.count[1][1][lane % kPickWaves] : 0);
+  const int above_all = __builtin_amdgcn_readlane(above_before, kPickWaves - 1);
+  int above_at = above_to - above + (wave > 0 ? __builtin_amdgcn_readlane(above_before, max(wave, 1) - 1) : 0);
+  int ties_at = ties_to - ties + (wave > 0 ? __builtin_amdgcn_readlane(ties_before, max(wave, 1) - 1) : 0);
+  const int room = kept - above_all;  // for keys equal to the smallest
+  for (int p = p0; p < p1; ++p) {
+    const bool pinned = p < free0 || p >= free1;
+    const uint32_t k = pinned ? 0 : key(p);
+    const bool over = pinned || k > least, tie = !pinned && k == least;
+    const int at = above_at + min(ties_at, room);
+    if (over || (tie && ties_at < room)) out[at] = table[p];
+    above_at += over ? 1 : 0;
+    ties_at += tie ? 1 : 0;
+  }
+}
+
+// A unit's length, and its output where every page is kept.
+__device__ __forceinline__ bool keep_all(const SelectArgs& a, int64_t unit, int b, int len, int pages) {
+  const int kept = min(pages, a.keep);
   if (threadIdx.x == 0) a.out_lens[unit] = kept > 0 ? (kept - 1) * a.page + (len - (pages - 1) * a.page) : 0;
-  if (pages <= a.keep) {
-    for (int i = threadIdx.x; i < pages; i += kPickThreads) out[i] = table[i];
-    return;
+  if (pages > a.keep) return false;
+  const int32_t* table = a.table + b * a.bt_stride;
+  for (int i = threadIdx.x; i < a.keep; i += blockDim.x) a.out_table[unit * a.keep + i] = i < pages ? table[i] : 0;
+  return true;
+}
+
+// Pages whose keys fit LDS.
+constexpr int kLdsPages = 8192;
+
+// A workgroup per (sequence, KV head): all steps.
+template <typename E, int D>
+__global__ void __launch_bounds__(kPickThreads) select_kernel(const SelectArgs a) {
+  __shared__ PickLds lds;
+  __shared__ uint32_t keys[kLdsPages];
+  const int64_t unit = blockIdx.x;
+  const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
+  const int len = select_len(a, b);
+  const int pages = (len + a.page - 1) / a.page;
+  if (keep_all(a, unit, b, len, pages)) return;
+  clear(lds);
+  const float scale = score_unit<E, D>(a, unit, b, h, pages, wave_id(), kPickWaves, keys);
+  pick_pages<E, D>(a, lds, unit, b, h, pages, keys, scale);
+}
+
+// Steps 2 and 3 from the keys of score_kernel.
+template <typename E, int D>
+__global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) {
+  __shared__ PickLds lds;
+  __shared__ uint32_t keys[kLdsPages];
+  const int64_t unit = blockIdx.x;
+  const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
+  const int len = select_len(a, b);
+  const int pages = (len + a.page - 1) / a.page;
+  if (keep_all(a, unit, b, len, pages)) return;
+  clear(lds);
+  uint32_t* from = a.keys + unit * a.max_pages;
+  const bool local = pages <= kLdsPages;
+  float scale = 0.0f;
+  for (int p = threadIdx.x; p < pages; p += kPickThreads) {
+    scale = fmaxf(scale, a.scale[static_cast<int64_t>(a.table[b * a.bt_stride + p]) * a.heads + h]);
+    if (local) keys[p] = from[p];
   }
-  auto key_of = [&](int p) -> uint32_t {
-    return p < a.first || p >= pages - a.last ? 0xffffffffu : score_key(scores[p]);
-  };
-  uint32_t prefix = 0;
-  int want = kept;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    hist[threadIdx.x] = 0;
-    __syncthreads();
-    for (int p = threadIdx.x; p < pages; p += kPickThreads) {
-      const uint32_t key = key_of(p);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255u], 1);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int left = want, bin = 255;
-      while (bin > 0 && hist[bin] < left) left -= hist[bin--];
-      s_prefix = prefix | (static_cast<uint32_t>(bin) << shift);
-      s_want = left;
-    }
-    __syncthreads();
-    prefix = s_prefix;
-    want = s_want;
-    __syncthreads();
+  if (local) {
+    pick_pages<E, D>(a, lds, unit, b, h, pages, keys, scale);
+  } else {
+    pick_pages<E, D>(a, lds, unit, b, h, pages, from, scale);
   }
-  // prefix is now the smallest key kept, `want` how many pages that have it.
-  const int lane = __lane_id(), wave = wave_id();
-  int done = 0, ties = 0;
-  for (int p0 = 0; p0 < pages; p0 += kPickThreads) {
-    const int p = p0 + threadIdx.x;
-    const uint32_t key = p < pages ? key_of(p) : 0;
-    const bool tie = p < pages && key == prefix;
-    const uint64_t tie_mask = __ballot(tie);
-    if (lane == 0) wave_count[0][wave] = __builtin_popcountll(tie_mask);
-    __syncthreads();
-    int ties_before = ties;
-    for (int w = 0; w < kPickThreads / 64; ++w) {
-      if (w < wave) ties_before += wave_count[0][w];
-      ties += wave_count[0][w];
-    }
-    const uint64_t below = (1ull << lane) - 1;
-    const bool take = (p < pages && key > prefix) || (tie && ties_before + __builtin_popcountll(tie_mask & below) < want);
-    const uint64_t mask = __ballot(take);
-    if (lane == 0) wave_count[1][wave] = __builtin_popcountll(mask);
-    __syncthreads();
-    int at = done + __builtin_popcountll(mask & below);
-    for (int w = 0; w < kPickThreads / 64; ++w) {
-      if (w < wave) at += wave_count[1][w];
-      done += wave_count[1][w];
-    }
-    if (take && at < a.keep) out[at] = table[p];
-    __syncthreads();
+}
+
+// Whether one launch does both. A workgroup of it takes a sequence and KV head from
+// end to end, so it suits tables that its 16 waves cover in a few tiles each, and any
+// that fits when the units fill the device; otherwise the scores are spread over the
+// device first.
+constexpr int kOneLaunchPages = 2048;
+bool one_launch(int64_t units, int max_pages) {
+  return max_pages <= kOneLaunchPages || (max_pages <= kLdsPages && units >= current_cu_count());
+}
+
+template <typename E, int D>
+int launch_select(const SelectArgs& a, int64_t units, hipStream_t stream) {
+  if (one_launch(units, a.max_pages)) {
+    select_kernel<E, D><<<static_cast<unsigned>(units), kPickThreads, 0, stream>>>(a);
+    return check_launch("select_pages kernel launch");
   }
+  if (a.max_pages > a.keep) {  // else every page is kept
+    // About four tiles a wave.
+    const dim3 grid(static_cast<unsigned>(cdiv(a.max_pages, 16 * 4 * kScoreWaves)), static_cast<unsigned>(units));
+    score_kernel<E, D><<<grid, kScoreWaves * 64, 0, stream>>>(a);
+    const int st = check_launch("select_pages score kernel launch");
+    if (st != KL_OK) return st;
+  }
+  pick_kernel<E, D><<<static_cast<unsigned>(units), kPickThreads, 0, stream>>>(a);
+  return check_launch("select_pages kernel launch");
+}
+
+template <typename E>
+int dispatch_select(const SelectArgs& a, int dim, int64_t units, hipStream_t stream) {
+  return dim == 64    ? launch_select<E, 64>(a, units, stream)
+         : dim == 128 ? launch_select<E, 128>(a, units, stream)
+                      : launch_select<E, 256>(a, units, stream);
 }
 
 bool head_dim_ok(int dim) { return dim == 64 || dim == 128 || dim == 256; }
@@ -601,8 +995,9 @@ extern "C" int kl_select_pages_workspace(int batch, int num_kv_heads, int max_pa
   if (batch < 0 || num_kv_heads <= 0 || max_pages < 0) {
     return fail(KL_ERR_INVALID_ARGUMENT, "batch, num_kv_heads and max_pages must be positive");
   }
+  const int64_t units = static_cast<int64_t>(batch) * num_kv_heads;
   if (out_workspace) {
-    *out_workspace = static_cast<size_t>(batch) * static_cast<size_t>(num_kv_heads) * static_cast<size_t>(max_pages) * 4;
+    *out_workspace = one_launch(units, max_pages) ? 0 : static_cast<size_t>(units) * static_cast<size_t>(max_pages) * 4;
   }
   return ok();
 }
@@ -642,9 +1037,12 @@ extern "C" int kl_select_pages(kl_dtype dtype, int32_t* out_table, int32_t* out_
   if (block_table_stride < max_pages && batch > 1) {
     return fail(KL_ERR_INVALID_ARGUMENT, "block_table_stride must be >= max_pages");
   }
+  if (reinterpret_cast<uintptr_t>(k_bounds) % 16 != 0) {
+    return fail(KL_ERR_INVALID_ARGUMENT, "k_bounds must be 16-byte aligned");
+  }
   size_t need = 0;
   kl_select_pages_workspace(batch, num_kv_heads, max_pages, &need);
-  if (workspace == nullptr || workspace_bytes < need) {
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
     return fail(KL_ERR_WORKSPACE, "workspace smaller than kl_select_pages_workspace reported");
   }
   SelectArgs a;
@@ -654,29 +1052,17 @@ extern "C" int kl_select_pages(kl_dtype dtype, int32_t* out_table, int32_t* out_
   a.table = block_table;
   a.seq_lens = seq_lens;
   a.bt_stride = block_table_stride;
-  a.scores = static_cast<float*>(workspace);
+  a.keys = static_cast<uint32_t*>(workspace);
   a.out_table = out_table;
   a.out_lens = out_lens;
   a.batch = batch;
   a.heads = num_kv_heads;
   a.group = num_q_heads / num_kv_heads;
-  a.dim = head_dim;
   a.page = page_size;
   a.max_pages = max_pages;
   a.keep = num_selected;
   a.first = first_pages;
   a.last = last_pages;
   const auto s = reinterpret_cast<hipStream_t>(stream);
-  if (max_pages > num_selected) {  // else every page is kept
-    const dim3 grid(static_cast<unsigned>(cdiv(max_pages, 4)), static_cast<unsigned>(units));
-    if (dtype == KL_DTYPE_F16) {
-      score_kernel<F16><<<grid, 256, 0, s>>>(a);
-    } else {
-      score_kernel<BF16><<<grid, 256, 0, s>>>(a);
-    }
-    const int st = check_launch("select_pages score kernel launch");
-    if (st != KL_OK) return st;
-  }
-  pick_kernel<<<static_cast<unsigned>(units), kPickThreads, 0, s>>>(a);
-  return check_launch("select_pages kernel launch");
+  return dtype == KL_DTYPE_F16 ? dispatch_select<F16>(a, head_dim, units, s) : dispatch_select<BF16>(a, head_dim, units, s);
 }

@@ -494,14 +494,15 @@ void select_pages(at::Tensor& out_table, at::Tensor& out_lens, const at::Tensor&
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   size_t ws_bytes = 0;
   check_status(kl_select_pages_workspace(b, heads, pages, &ws_bytes), "select_pages planning");
-  at::Tensor workspace = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+  at::Tensor workspace;
+  if (ws_bytes > 0) workspace = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
   check_status(
       kl_select_pages(to_kl_dtype(q.scalar_type()), out_table.data_ptr<int32_t>(), out_lens.data_ptr<int32_t>(),
                       q.data_ptr(), k_bounds.data_ptr(), k_scale.data_ptr<float>(), block_table.data_ptr<int32_t>(),
                       seq_lens.data_ptr<int32_t>(), b, checked_int(hq, "num_q_heads"), heads,
                       checked_int(q.size(2), "head_dim"), checked_int(page_size, "page_size"), bt_stride, pages,
                       checked_int(keep, "num_selected"), checked_int(first_pages, "first_pages"),
-                      checked_int(last_pages, "last_pages"), workspace.data_ptr(), ws_bytes, current_stream(dev)),
+                      checked_int(last_pages, "last_pages"), ws_bytes > 0 ? workspace.data_ptr() : nullptr, ws_bytes, current_stream(dev)),
       "select_pages");
 }
 

@@ -118,10 +118,51 @@ def test_near_scores_are_told_apart(gpu_ops):
     check(gpu_ops, q, edges, torch.ones(pages, 1), table, torch.tensor([16 * pages], dtype=torch.int32), 20, 16, first=0)
 
 
+@pytest.mark.parametrize(("dtype", "size"), [(torch.float16, 2.0**-20), (torch.float16, 2.0**-16), (torch.bfloat16, 1e-39), (torch.bfloat16, 1e-30),
+                                             (torch.bfloat16, 1e30), (torch.float16, 1e4)])
+def test_queries_far_from_one(gpu_ops, dtype, size):
+    """Subnormal queries, and sums near the end of float32's range."""
+    q, edges, scale, table, lens = problem([16 * 300, 16 * 90], 8, 2, 128, torch.float32, 16, seed=6)
+    check(gpu_ops, (q * size).to(dtype), edges, scale, table, lens, 20, 16)
+
+
+@pytest.mark.parametrize("pages", [300, 1500])
+def test_many_pages_between(gpu_ops, pages):
+    """Scores so near one another that the 16-bit matrix cores' sums cannot order them: hundreds are scored in 64 bits."""
+    q, edges, scale, table, lens = problem([16 * pages], 8, 2, 128, torch.bfloat16, 16, seed=7)
+    g = torch.Generator().manual_seed(1)
+    edges.copy_(edges[:1].float().nan_to_num(1.0).to(F8).expand_as(edges))
+    scale.copy_((1 + 1e-6 * torch.randn(scale.shape, generator=g)) * 0.01)
+    check(gpu_ops, q, edges, scale, table, lens, 100, 16)
+    edges[:, :, :, 3] = torch.rand(edges.shape[0], 2, 1, generator=g).expand(-1, -1, 2).to(F8)
+    check(gpu_ops, q, edges, scale, table, lens, 100, 16)
+
+
 def test_lengths_past_the_table_and_below_zero(gpu_ops):
     q, edges, scale, table, lens = problem([16 * 30, 16 * 30, 16 * 30], 8, 2, 64, torch.bfloat16, 16)
     lens = torch.tensor([16 * 30 + 100, -5, 2**31 - 1], dtype=torch.int32)
     check(gpu_ops, q, edges, scale, table, lens, 8, 16)
+
+
+@pytest.mark.parametrize(("pages", "group"), [(2048, 4), (2049, 4), (2300, 8), (3000, 16), (2100, 40), (8192, 1), (9000, 2)])
+def test_long_tables_of_few_sequences(gpu_ops, pages, group):
+    """Past what one workgroup scores: the scores get a launch of their own; past its LDS, the keys stay in memory."""
+    lens = [16 * pages - 3, 16 * 100, 5]
+    args = problem(lens, group, 1, 64, torch.bfloat16, 16, seed=pages)
+    check(gpu_ops, *args, 64, 16)
+    check(gpu_ops, *args, 2047, 16, first=3, last=2)
+
+
+def test_long_tables_of_a_full_batch(gpu_ops):
+    """As many (sequence, KV head) pairs as compute units: one launch up to its LDS."""
+    lens = torch.randint(0, 16 * 2500, (64,), generator=torch.Generator().manual_seed(2)).tolist()
+    lens[3] = 16 * 2500
+    args = problem(lens, 8, 4, 64, torch.float16, 16, seed=4)
+    q, edges, scale, table, lens = args
+    got = gpu_ops.select_pages(q.cuda(), edges.cuda(), scale.cuda(), table.cuda(), lens.cuda(), 40, 16)
+    rows = [0, 3, 17, 63]
+    want = ref.select(q[rows], edges, scale, table[rows], lens[rows], 40, 16)
+    assert torch.equal(got[0].cpu()[rows], want[0]) and torch.equal(got[1].cpu()[rows], want[1])
 
 
 def test_strided_table(gpu_ops):
@@ -181,23 +222,26 @@ def test_graph_replays(gpu_ops):
         assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
 
 
-def test_through_c_abi(gpu_ops):
+@pytest.mark.parametrize("pages", [90, 2500])
+def test_through_c_abi(gpu_ops, pages):
+    """A table that one launch serves without a workspace, and one whose scores need it."""
     lib = _native.core()
-    host = problem([16 * 90, 16 * 40 + 3], 16, 4, 128, torch.bfloat16, 16)
+    host = problem([16 * pages, 16 * 40 + 3], 16, 4, 128, torch.bfloat16, 16)
     q, edges, scale, table, lens = (t.cuda() for t in host)
     ws = ctypes.c_size_t(0)
-    assert lib.kl_select_pages_workspace(2, 4, 90, ctypes.byref(ws)) == 0 and ws.value >= 2 * 4 * 90 * 4
-    work = torch.empty(ws.value, dtype=torch.uint8, device="cuda")
+    assert lib.kl_select_pages_workspace(2, 4, pages, ctypes.byref(ws)) == 0 and ws.value == (0 if pages == 90 else 2 * 4 * pages * 4)
+    work = torch.empty(max(1, ws.value), dtype=torch.uint8, device="cuda")
     out, out_lens = torch.empty(2, 4, 12, dtype=torch.int32, device="cuda"), torch.empty(2, 4, dtype=torch.int32, device="cuda")
 
     def call(bytes_=ws.value, first=1):
         return lib.kl_select_pages(2, out.data_ptr(), out_lens.data_ptr(), q.data_ptr(), edges.data_ptr(), scale.data_ptr(),
-                                   table.data_ptr(), lens.data_ptr(), 2, 16, 4, 128, 16, 90, 90, 12, first, 1, work.data_ptr(),
+                                   table.data_ptr(), lens.data_ptr(), 2, 16, 4, 128, 16, pages, pages, 12, first, 1, work.data_ptr(),
                                    bytes_, torch.cuda.current_stream().cuda_stream)
 
     assert call() == 0, _native.last_error()
     torch.cuda.synchronize()
     want = ref.select(*host, 12, 16)
     assert torch.equal(out.cpu(), want[0]) and torch.equal(out_lens.cpu(), want[1])
-    assert call(bytes_=ws.value - 4) == 3
+    if ws.value:
+        assert call(bytes_=ws.value - 4) == 3
     assert call(first=12) == 1
