@@ -405,6 +405,8 @@ int launch_append(AppendArgs& a, int64_t tiles, hipStream_t stream) {
 //   3. scores in 64 bits for the pages between (some ten of a thousand), and the choice
 //      among them.
 // Where a score is not finite, every page is one between.
+constexpr int kTile = 16;  // pages that a wave scores at once
+
 struct SelectArgs {
   const void* q;
   const uint8_t* bounds;
@@ -412,11 +414,19 @@ struct SelectArgs {
   const int32_t* table;
   const int32_t* seq_lens;
   int64_t bt_stride;
-  uint32_t* keys;  // [batch, kv heads, max_pages], where the scores have a launch of their own
+  // Where a unit's scores come from several workgroups, of each unit: its pages' keys,
+  // then each tile's largest k_scale.
+  uint32_t* keys;
+  uint32_t* arrivals;  // a counter a unit, zero and left zero; null: none
   int32_t* out_table;
   int32_t* out_lens;
   int batch, heads, group, page, max_pages, keep, first, last;
 };
+
+// Words of a unit in SelectArgs::keys.
+__host__ __device__ __forceinline__ int64_t unit_words(int64_t max_pages) {
+  return max_pages + (max_pages + kTile - 1) / kTile;
+}
 
 __device__ __forceinline__ int select_len(const SelectArgs& a, int b) {
   const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page;
@@ -450,10 +460,11 @@ __device__ __forceinline__ double dpp64(double v) {
 // The larger of two, NaN if either is.
 __device__ __forceinline__ double max_or_nan(double a, double b) { return a != a || a > b ? a : b; }
 
-// 16-bit matrix products: 16 pages by 16 query heads, 32 bytes of the bounds a step.
-// Lane l supplies A[page l % 16] and B[head l % 16] for eight k of group l / 16 and gets
-// the scores of pages 4 (l / 16) .. + 3 and head l % 16. Which bytes a step's k are is
-// free as long as A and B agree: a lane's load of 16 codes is its eight k of two steps.
+// 16-bit matrix products: 16 query heads by 16 pages, 32 bytes of the bounds a step.
+// Lane l supplies A[head l % 16] and B[page l % 16] for eight k of group l / 16 and gets
+// the scores of heads 4 (l / 16) .. + 3 and page l % 16, so up to four heads need no
+// reduction over lanes. Which bytes a step's k are is free as long as A and B agree: a
+// lane's load of 16 codes is its eight k of two steps.
 template <typename E>
 __device__ __forceinline__ f32x4 score_mma(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (std::is_same_v<E, F16>) {
@@ -465,7 +476,7 @@ __device__ __forceinline__ f32x4 score_mma(u32x4 a, u32x4 b, f32x4 c) {
 
 constexpr int kHeadsAtOnce = 16;
 
-// Query heads g0 .. g0 + 15 of a unit as the B operands, heads past the group as zeros:
+// Query heads g0 .. g0 + 15 of a unit as the A operands, heads past the group as zeros:
 // lane l's eight values of step 2 c + half are byte 64 c + 16 (l / 16) + 8 half of
 // [lo hi] on, so min(q, 0) in the first half of the steps and max(q, 0) in the others.
 template <typename E, int D>
@@ -493,65 +504,57 @@ struct ScoreQueries {
   }
 };
 
-// The keys, from step 1's scores, of pages 16 tile .. 16 tile + 15 of a unit, by a
-// wave: store(page, key). Returns the largest k_scale that the lane has seen.
-template <typename E, int D, typename Store>
-__device__ __forceinline__ float score_tile(const SelectArgs& a, const ScoreQueries<E, D>& q, int b, int h, int g0,
-                                            int pages, int tile, Store&& store) {
-  constexpr int C = 2 * D / 64;
+// Step 1 for a unit's tiles first, first + step, ..., by a wave: store(page, key) by lanes
+// 0 .. 15, and scale(tile, largest k_scale of its pages) in every lane.
+//
+// What bounds it: the bounds of a unit arrive at a CU's share of HBM bandwidth, 256 KiB
+// for 1,024 pages of head_dim 128 (11 us on one CU), so a unit's tiles are spread over
+// several workgroups. Loading a tile ahead gained nothing.
+template <typename E, int D, typename Store, typename Scale>
+__device__ __forceinline__ void score_unit(const SelectArgs& a, int64_t unit, int b, int h, int pages, int first,
+                                           int step, Store&& store, Scale&& tile_scale) {
+  constexpr int C = 2 * D / 64;  // loads of 16 bytes a lane for a tile
   const int lane = __lane_id(), k = lane >> 4;
+  const int tiles = (pages + kTile - 1) / kTile;
+  if (first >= tiles) return;
   const int32_t* table = a.table + b * a.bt_stride;
-  const int phys = table[min(16 * tile + (lane & 15), pages - 1)];
-  const int64_t head = static_cast<int64_t>(phys) * a.heads + h;
-  const uint8_t* edge = a.bounds + head * (2 * D) + 16 * k;
-  u32x4 w[C];
+  ScoreQueries<E, D> q(a, unit, 0);
+  for (int tile = first; tile < tiles; tile += step) {
+    const int page = kTile * tile + (lane & 15);
+    const int64_t head = static_cast<int64_t>(table[min(page, pages - 1)]) * a.heads + h;
+    const uint8_t* edge = a.bounds + head * (2 * D) + 16 * k;
+    u32x4 w[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) w[c] = *reinterpret_cast<const u32x4*>(edge + 64 * c);
-  const float scale = a.scale[head];
-  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < C; ++c) w[c] = *reinterpret_cast<const u32x4*>(edge + 64 * c);
+    const float scale = a.scale[head];
+    float best = -INFINITY;
+    bool finite = true;
+    for (int g0 = 0; g0 < a.group; g0 += kHeadsAtOnce) {
+      if (a.group > kHeadsAtOnce) q = ScoreQueries<E, D>(a, unit, g0);
+      f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    u32x4 lo, hi;
-    fp8x16_to<E>(w[c], lo, hi);
-    s = score_mma<E>(lo, q.v[c][0], s);
-    s = score_mma<E>(hi, q.v[c][1], s);
-  }
-  // Lane 4 k + i of the 16 gets page 4 k + i's score; a maximum drops a NaN, a sum keeps it.
-  const bool valid = g0 + (lane & 15) < a.group;
-  float mine = 0.0f, check = 0.0f;
+      for (int c = 0; c < C; ++c) {
+        u32x4 lo, hi;
+        fp8x16_to<E>(w[c], lo, hi);
+        sum = score_mma<E>(q.v[c][0], lo, sum);
+        sum = score_mma<E>(q.v[c][1], hi, sum);
+      }
+      // Lane l has heads 4 k .. + 3 of page l % 16.
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float m = row16_max(valid ? s[i] : -INFINITY), n = row16_sum(valid ? s[i] * 0.0f : 0.0f);
-    if ((lane & 3) == i) {
-      mine = m;
-      check = n;
+      for (int i = 0; i < 4; ++i) {
+        const bool valid = g0 + 4 * k + i < a.group;
+        finite &= !valid || fabsf(sum[i]) < INFINITY;
+        best = valid ? fmaxf(best, sum[i]) : best;
+      }
     }
+    if (a.group > 4) best = max_xor32(max_xor16(best));
+    const float score = best * scale;
+    finite &= k > 0 || fabsf(score) < INFINITY;
+    // A score that is not finite marks its tile, and so the unit.
+    const uint32_t key = __any(!finite) ? kKeyNotFinite : score_key(score);
+    if (k == 0 && page < pages) store(page, key);
+    tile_scale(tile, row16_max(scale));
   }
-  const int m = 4 * k + (lane & 3);
-  const float m_scale = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * m, __builtin_bit_cast(int, scale)));
-  const float score = mine * m_scale + check;
-  const int page = 16 * tile + m;
-  if ((lane & 15) < 4 && page < pages) store(page, fabsf(score) < INFINITY ? score_key(score) : kKeyNotFinite);
-  return scale;
-}
-
-// Keys of tiles first, first + step, ... of a unit into keys[page], by a wave. Groups of
-// more than kHeadsAtOnce heads take several rounds: a scale is not negative, so the
-// maximum over heads may be taken after the product with it.
-template <typename E, int D>
-__device__ __forceinline__ float score_unit(const SelectArgs& a, int64_t unit, int b, int h, int pages, int first,
-                                            int step, uint32_t* keys) {
-  const int tiles = (pages + 15) / 16;
-  float most = 0.0f;
-  for (int g0 = 0; g0 < a.group; g0 += kHeadsAtOnce) {
-    const ScoreQueries<E, D> q(a, unit, g0);
-    for (int tile = first; tile < tiles; tile += step) {
-      most = fmaxf(most, score_tile<E, D>(a, q, b, h, g0, pages, tile, [&](int page, uint32_t key) {
-                     keys[page] = g0 == 0 ? key : max(keys[page], key);
-                   }));
-    }
-  }
-  return most;
 }
 
 // How far step 1's score may be from the true one, over the sum of its terms' sizes: a
@@ -602,29 +605,15 @@ __device__ __forceinline__ uint32_t true_key(const SelectArgs& a, int64_t unit, 
   return score_key(static_cast<float>(best * scale));
 }
 
-constexpr int kScoreWaves = 4;
-
-// Step 1 in a launch of its own: workgroups along x share a unit's tiles.
-template <typename E, int D>
-__global__ void __launch_bounds__(kScoreWaves * 64) score_kernel(const SelectArgs a) {
-  const int64_t unit = blockIdx.y;
-  const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
-  const int pages = (select_len(a, b) + a.page - 1) / a.page;
-  const int first = static_cast<int>(blockIdx.x) * kScoreWaves + wave_id();
-  if (16 * first >= pages || pages <= a.keep) return;
-  score_unit<E, D>(a, unit, b, h, pages, first, kScoreWaves * static_cast<int>(gridDim.x), a.keys + unit * a.max_pages);
-}
-
-constexpr int kPickWaves = 16;
-constexpr int kPickThreads = kPickWaves * 64;
-
-constexpr int kBins = kPickThreads;
+// Workgroups of W waves (W = 8 or 16: see wide_workgroups).
 constexpr int kListed = 64;  // pages between that a wave ranks
 
+template <int W>
 struct PickLds {
-  int count[2][3][kPickWaves];  // of two rounds in turn, so that a round needs one barrier
-  float scale[kPickWaves], size[kPickWaves];
-  uint32_t low[kPickWaves], high[kPickWaves];
+  static constexpr int kBins = 64 * W;
+  int count[2][3][W];  // of two rounds in turn, so that a round needs one barrier
+  float scale[W], size[W];
+  uint32_t low[W], high[W];
   int bins[kBins];
   int bin;                    // that holds T
   int kept, between;          // pages certainly kept, pages between
@@ -633,28 +622,29 @@ struct PickLds {
 };
 
 // Before the first barrier of pick_pages.
-__device__ __forceinline__ void clear(PickLds& lds) {
+template <int W>
+__device__ __forceinline__ void clear(PickLds<W>& lds) {
   lds.bins[threadIdx.x] = 0;
   if (threadIdx.x == 0) lds.kept = lds.between = 0;
 }
 
-// The smallest of the `want` largest keys of pages [q0, q1) of all threads, by a
-// workgroup of kPickThreads.
+// The smallest of the `want` largest keys of pages q0, q0 + 64 W, ... < free1 of all
+// threads, by a workgroup.
 //
 // The interval that holds it is cut in four: each round counts the keys from three
 // thresholds on. It ends as soon as a threshold leaves exactly the number wanted, after
 // about half of log2(pages) rounds beyond the bits that all keys share; only equal keys
 // take it to the end. For selections that have many pages between (equal or nearly
 // equal scores): a round's counts go through LDS, and 15 of them took 20 us.
-template <typename Key>
-__device__ uint32_t smallest_kept(PickLds& lds, int want, int q0, int q1, uint32_t low, uint32_t high, Key&& key) {
+template <int W, typename Key>
+__device__ uint32_t smallest_kept(PickLds<W>& lds, int want, int q0, int free1, uint32_t low, uint32_t high, Key&& key) {
   const int wave = wave_id(), lane = __lane_id();
   // Keys from `low` on are `want` at least, from high + 1 on fewer.
   for (int round = 0; low < high; ++round) {
     const uint32_t step = (high - low) / 4;
     const uint32_t t[3] = {low + step + 1, low + 2 * step + 1, low + 3 * step + 1};
     int n[3] = {0, 0, 0};
-    for (int p = q0; p < q1; ++p) {
+    for (int p = q0; p < free1; p += 64 * W) {
       const uint32_t k = key(p);
 #pragma unroll
       for (int i = 0; i < 3; ++i) n[i] += k >= t[i] ? 1 : 0;
@@ -668,7 +658,7 @@ __device__ uint32_t smallest_kept(PickLds& lds, int want, int q0, int q1, uint32
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
       n[i] = 0;
-      for (int w = 0; w < kPickWaves; ++w) n[i] += lds.count[round & 1][i][w];
+      for (int w = 0; w < W; ++w) n[i] += lds.count[round & 1][i][w];
     }
     const int side = n[2] >= want ? 3 : n[1] >= want ? 2 : n[0] >= want ? 1 : 0;
     if (side < 3) high = t[side] - 1;
@@ -681,32 +671,30 @@ __device__ uint32_t smallest_kept(PickLds& lds, int want, int q0, int q1, uint32
   return low;
 }
 
-// Steps 2 and 3, by a workgroup of kPickThreads: a unit's pages from its keys. scale: the
+// Steps 2 and 3, by a workgroup: a unit's pages from its keys. scale: the
 // largest k_scale that the lane has seen of the unit's pages.
-template <typename E, int D>
-__device__ void pick_pages(const SelectArgs& a, PickLds& lds, int64_t unit, int b, int h, int pages, uint32_t* keys,
+template <typename E, int D, int W>
+__device__ void pick_pages(const SelectArgs& a, PickLds<W>& lds, int64_t unit, int b, int h, int pages, uint32_t* keys,
                            float scale) {
+  constexpr int kBins = PickLds<W>::kBins;
   const int wave = wave_id(), lane = __lane_id();
   const int kept = a.keep;  // < pages
   const int32_t* table = a.table + b * a.bt_stride;
   int32_t* out = a.out_table + unit * a.keep;
-  // A thread's pages are neighbours, so that ranks in the sequence are prefix sums.
-  const int each = (pages + kPickThreads - 1) / kPickThreads;
-  const int p0 = min(static_cast<int>(threadIdx.x) * each, pages), p1 = min(p0 + each, pages);
   const int free0 = a.first, free1 = pages - a.last;  // pages that are not pinned
-  const int q0 = max(p0, free0), q1 = min(p1, free1);
+  const int q0 = free0 + static_cast<int>(threadIdx.x);
   const int want = kept - a.first - a.last;
   auto key = [&](int p) { return keys[p]; };
 
   scale = max_xor32(max_xor16(row16_max(scale)));
-  const float size = query_size<E, D>(a, unit, wave, kPickWaves);
+  const float size = query_size<E, D>(a, unit, wave, W);
   if (lane == 0) {
     lds.scale[wave] = scale;
     lds.size[wave] = size;
   }
   __syncthreads();  // the keys are there, too
   uint32_t low = 0xffffffffu, high = 0;
-  for (int p = q0; p < q1; ++p) {
+  for (int p = q0; p < free1; p += 64 * W) {
     low = min(low, key(p));
     high = max(high, key(p));
   }
@@ -719,11 +707,11 @@ __device__ void pick_pages(const SelectArgs& a, PickLds& lds, int64_t unit, int 
     lds.high[wave] = high;
   }
   __syncthreads();
-  low = lds.low[lane % kPickWaves];
-  high = lds.high[lane % kPickWaves];
-  scale = row16_max(lds.scale[lane % kPickWaves]);
-  const float most_size = row16_max(lds.size[lane % kPickWaves]);
-  for (int m = 8; m > 0; m >>= 1) {
+  low = lds.low[lane % W];
+  high = lds.high[lane % W];
+  scale = row16_max(lds.scale[lane % W]);
+  const float most_size = row16_max(lds.size[lane % W]);
+  for (int m = W / 2; m > 0; m >>= 1) {
     low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), m)));
     high = max(high, static_cast<uint32_t>(__shfl_xor(static_cast<int>(high), m)));
   }
@@ -738,14 +726,14 @@ __device__ void pick_pages(const SelectArgs& a, PickLds& lds, int64_t unit, int 
     auto bin_of = [&](float s) { return static_cast<int>(fminf(fmaxf((s - lowest) * to_bin, -1.0f), 1.0f * kBins)); };
     int bin = 0;
     if (finite) {
-      for (int p = q0; p < q1; ++p) atomicAdd(&lds.bins[min(bin_of(key_score(key(p))), kBins - 1)], 1);
+      for (int p = q0; p < free1; p += 64 * W) atomicAdd(&lds.bins[min(bin_of(key_score(key(p))), kBins - 1)], 1);
       __syncthreads();
       // Thread t has bin kBins - 1 - t; the pages from it upwards.
       const int mine = lds.bins[kBins - 1 - static_cast<int>(threadIdx.x)];
       int upto = wave_prefix_sum(mine);
       if (lane == 63) lds.count[0][0][wave] = upto;
       __syncthreads();
-      const int ahead = lane < wave ? lds.count[0][0][lane % kPickWaves] : 0;
+      const int ahead = lane < wave ? lds.count[0][0][lane % W] : 0;
       upto += __builtin_amdgcn_readlane(wave_prefix_sum(ahead), 63);
       if (upto >= want && upto - mine < want) lds.bin = kBins - 1 - static_cast<int>(threadIdx.x);
       __syncthreads();
@@ -753,7 +741,7 @@ __device__ void pick_pages(const SelectArgs& a, PickLds& lds, int64_t unit, int 
     }
     // Step 3. The pages between are listed in the order that they come in; which of them
     // are kept does not depend on it. (The last bin takes what is past its end, too.)
-    for (int p = q0; p < q1; ++p) {
+    for (int p = q0; p < free1; p += 64 * W) {
       const float s = key_score(key(p));
       if (finite && bin < kBins - 1 && bin_of(s - reach) > bin) {
         keys[p] = kKeyKept;
@@ -769,7 +757,7 @@ __device__ void pick_pages(const SelectArgs& a, PickLds& lds, int64_t unit, int 
     __syncthreads();
     const int between = lds.between;
     if (between <= kListed) {
-      for (int i = wave; i < between; i += kPickWaves) {
+      for (int i = wave; i < between; i += W) {
         const uint32_t k = true_key<E, D>(a, unit, b, h, __builtin_amdgcn_readfirstlane(lds.list[i]));
         if (lane == 0) lds.list_key[i] = k;
       }
@@ -789,7 +777,7 @@ __device__ void pick_pages(const SelectArgs& a, PickLds& lds, int64_t unit, int 
       __syncthreads();
       least = kKeyKept;
     } else {
-      for (int base = wave * 64; base < pages; base += kPickThreads) {
+      for (int base = wave * 64; base < pages; base += 64 * W) {
         const int p = base + lane;
         uint64_t todo = __ballot(p >= free0 && p < free1 && keys[min(p, pages - 1)] == kKeyNotFinite);
         for (; todo != 0; todo &= todo - 1) {
@@ -799,124 +787,214 @@ __device__ void pick_pages(const SelectArgs& a, PickLds& lds, int64_t unit, int 
         }
       }
       __syncthreads();
-      least = smallest_kept(lds, want, q0, q1, 0, kKeyKept, key);
+      least = smallest_kept(lds, want, q0, free1, 0, kKeyKept, key);
     }
   }
 
-  // Positions: pages above the smallest key kept, and the first ones equal to it.
-  int above = max(0, min(p1, free0) - p0) + max(0, p1 - max(p0, free1)), ties = 0;
-  for (int p = q0; p < q1; ++p) {
-    const uint32_t k = key(p);
-    above += k > least ? 1 : 0;
-    ties += k == least ? 1 : 0;
-  }
-  const int above_to = wave_prefix_sum(above), ties_to = wave_prefix_sum(ties);
-  if (lane == 63) {
-    lds.count[1][0][wave] = above_to;
-    lds.count[1][1][wave] = ties_to;
+  // Positions: pages above the smallest key kept, and the first ones equal to it. A wave
+  // has neighbouring pages, 64 at a time, whose ranks are counts of lanes below.
+  const int range = (pages + 64 * W - 1) / (64 * W) * 64;
+  const int p0 = min(wave * range, pages), p1 = min(p0 + range, pages);
+  auto ranked = [&](auto&& take) {
+    for (int base = p0; base < p1; base += 64) {
+      const int p = base + lane;
+      const bool pinned = p < free0 || p >= free1;
+      const uint32_t k = p < p1 && !pinned ? key(p) : 0;
+      take(p, __ballot(p < p1 && (pinned || k > least)), __ballot(p < p1 && !pinned && k == least));
+    }
+  };
+  int above = 0, ties = 0;
+  ranked([&](int, uint64_t over, uint64_t tie) {
+    above += __builtin_popcountll(over);
+    ties += __builtin_popcountll(tie);
+  });
+  if (lane == 0) {
+    lds.count[1][0][wave] = above;
+    lds.count[1][1][wave] = ties;
   }
   __syncthreads();
-  const int above_before = wave_prefix_sum(lane < kPickWaves ? lds.count[1][0][lane % kPickWaves] : 0);
-  const int ties_before = wave_prefix_sum(lane < kPickWaves ? lds.count[1][1][lane % kPickWaves] : 0);
-  const int above_all = __builtin_amdgcn_readlane(above_before, kPickWaves - 1);
-  int above_at = above_to - above + (wave > 0 ? __builtin_amdgcn_readlane(above_before, max(wave, 1) - 1) : 0);
-  int ties_at = ties_to - ties + (wave > 0 ? __builtin_amdgcn_readlane(ties_before, max(wave, 1) - 1) : 0);
-  const int room = kept - above_all;  // for keys equal to the smallest
-  for (int p = p0; p < p1; ++p) {
-    const bool pinned = p < free0 || p >= free1;
-    const uint32_t k = pinned ? 0 : key(p);
-    const bool over = pinned || k > least, tie = !pinned && k == least;
-    const int at = above_at + min(ties_at, room);
-    if (over || (tie && ties_at < room)) out[at] = table[p];
-    above_at += over ? 1 : 0;
-    ties_at += tie ? 1 : 0;
+  int above_at = 0, ties_at = 0, above_all = 0;
+  for (int w = 0; w < W; ++w) {
+    if (w < wave) {
+      above_at += lds.count[1][0][w];
+      ties_at += lds.count[1][1][w];
+    }
+    above_all += lds.count[1][0][w];
   }
+  const int room = kept - above_all;  // for keys equal to the smallest
+  const uint64_t below = (1ull << lane) - 1, mine = 1ull << lane;
+  ranked([&](int p, uint64_t over, uint64_t tie) {
+    const int ties_here = ties_at + __builtin_popcountll(tie & below);
+    const int at = above_at + __builtin_popcountll(over & below) + min(ties_here, room);
+    if ((over & mine) != 0 || ((tie & mine) != 0 && ties_here < room)) out[at] = table[p];
+    above_at += __builtin_popcountll(over);
+    ties_at += __builtin_popcountll(tie);
+  });
 }
 
-// A unit's length, and its output where every page is kept.
-__device__ __forceinline__ bool keep_all(const SelectArgs& a, int64_t unit, int b, int len, int pages) {
-  const int kept = min(pages, a.keep);
-  if (threadIdx.x == 0) a.out_lens[unit] = kept > 0 ? (kept - 1) * a.page + (len - (pages - 1) * a.page) : 0;
-  if (pages > a.keep) return false;
+// A unit's length, and its output where every page is kept, by one workgroup.
+__device__ __forceinline__ void keep_all(const SelectArgs& a, int64_t unit, int b, int pages) {
   const int32_t* table = a.table + b * a.bt_stride;
   for (int i = threadIdx.x; i < a.keep; i += blockDim.x) a.out_table[unit * a.keep + i] = i < pages ? table[i] : 0;
-  return true;
+}
+__device__ __forceinline__ void write_len(const SelectArgs& a, int64_t unit, int len, int pages) {
+  const int kept = min(pages, a.keep);
+  if (threadIdx.x == 0) a.out_lens[unit] = kept > 0 ? (kept - 1) * a.page + (len - (pages - 1) * a.page) : 0;
 }
 
 // Pages whose keys fit LDS.
 constexpr int kLdsPages = 8192;
 
-// A workgroup per (sequence, KV head): all steps.
-template <typename E, int D>
-__global__ void __launch_bounds__(kPickThreads) select_kernel(const SelectArgs a) {
-  __shared__ PickLds lds;
+// One launch for all steps. The workgroups along x share a unit's tiles; where more than
+// one has any, they leave keys and scales in memory, device-coherent, and the last to
+// arrive (paged_decode.hip's arrive_and_merge has the order of accesses) takes steps 2
+// and 3. At most kLdsPages pages a unit.
+template <typename E, int D, int W>
+__global__ void __launch_bounds__(64 * W) select_kernel(const SelectArgs a) {
+  __shared__ PickLds<W> lds;
   __shared__ uint32_t keys[kLdsPages];
-  const int64_t unit = blockIdx.x;
+  __shared__ int s_last;
+  const int64_t unit = blockIdx.y;
   const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
   const int len = select_len(a, b);
   const int pages = (len + a.page - 1) / a.page;
-  if (keep_all(a, unit, b, len, pages)) return;
+  const int tiles = (pages + kTile - 1) / kTile;
+  const int wgs = max(1, min(static_cast<int>(gridDim.x), (tiles + W - 1) / W));
+  if (pages <= a.keep) {
+    if (blockIdx.x == 0) {
+      write_len(a, unit, len, pages);
+      keep_all(a, unit, b, pages);
+    }
+    return;
+  }
+  if (static_cast<int>(blockIdx.x) >= wgs) return;
   clear(lds);
-  const float scale = score_unit<E, D>(a, unit, b, h, pages, wave_id(), kPickWaves, keys);
-  pick_pages<E, D>(a, lds, unit, b, h, pages, keys, scale);
-}
-
-// Steps 2 and 3 from the keys of score_kernel.
-template <typename E, int D>
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) {
-  __shared__ PickLds lds;
-  __shared__ uint32_t keys[kLdsPages];
-  const int64_t unit = blockIdx.x;
-  const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
-  const int len = select_len(a, b);
-  const int pages = (len + a.page - 1) / a.page;
-  if (keep_all(a, unit, b, len, pages)) return;
-  clear(lds);
-  uint32_t* from = a.keys + unit * a.max_pages;
-  const bool local = pages <= kLdsPages;
+  const int first = static_cast<int>(blockIdx.x) * W + wave_id(), step = wgs * W;
   float scale = 0.0f;
-  for (int p = threadIdx.x; p < pages; p += kPickThreads) {
-    scale = fmaxf(scale, a.scale[static_cast<int64_t>(a.table[b * a.bt_stride + p]) * a.heads + h]);
-    if (local) keys[p] = from[p];
-  }
-  if (local) {
-    pick_pages<E, D>(a, lds, unit, b, h, pages, keys, scale);
+  if (wgs == 1) {
+    score_unit<E, D>(a, unit, b, h, pages, first, step, [&](int page, uint32_t key) { keys[page] = key; },
+                     [&](int, float s) { scale = fmaxf(scale, s); });
   } else {
-    pick_pages<E, D>(a, lds, unit, b, h, pages, from, scale);
+    uint32_t* shared = a.keys + unit * unit_words(a.max_pages);
+    const auto rsrc = make_rsrc(uniform_ptr(shared));
+    score_unit<E, D>(
+        a, unit, b, h, pages, first, step,
+        [&](int page, uint32_t key) {
+          buffer_store_f32<kCachePolicyDevice>(rsrc, static_cast<uint32_t>(page) * 4u, __builtin_bit_cast(float, key));
+        },
+        [&](int tile, float s) {
+          if (__lane_id() == 0) {
+            buffer_store_f32<kCachePolicyDevice>(rsrc, static_cast<uint32_t>(a.max_pages + tile) * 4u, s);
+          }
+        });
+    wait_vector_memory();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const uint32_t old = __hip_atomic_fetch_add(a.arrivals + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_last = old + 1 == static_cast<uint32_t>(wgs);
+      if (s_last) __hip_atomic_store(a.arrivals + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!__builtin_amdgcn_readfirstlane(s_last)) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");  // no load moves above the arrival
+    for (int p = threadIdx.x; p < pages; p += 64 * W) {
+      keys[p] = __builtin_bit_cast(uint32_t, buffer_load_f32<kCachePolicyDevice>(rsrc, static_cast<uint32_t>(p) * 4u));
+    }
+    for (int t = threadIdx.x; t < tiles; t += 64 * W) {
+      scale = fmaxf(scale, buffer_load_f32<kCachePolicyDevice>(rsrc, static_cast<uint32_t>(a.max_pages + t) * 4u));
+    }
+  }
+  write_len(a, unit, len, pages);
+  pick_pages<E, D, W>(a, lds, unit, b, h, pages, keys, scale);
+}
+
+// The same in two launches: for tables past kLdsPages, and where there are no counters.
+template <typename E, int D, int W>
+__global__ void __launch_bounds__(64 * W) score_kernel(const SelectArgs a) {
+  const int64_t unit = blockIdx.y;
+  const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
+  const int pages = (select_len(a, b) + a.page - 1) / a.page;
+  if (pages <= a.keep) return;
+  uint32_t* shared = a.keys + unit * unit_words(a.max_pages);
+  score_unit<E, D>(a, unit, b, h, pages, static_cast<int>(blockIdx.x) * W + wave_id(),
+                   W * static_cast<int>(gridDim.x), [&](int page, uint32_t key) { shared[page] = key; },
+                   [&](int tile, float s) {
+                     if (__lane_id() == 0) shared[a.max_pages + tile] = __builtin_bit_cast(uint32_t, s);
+                   });
+}
+
+template <typename E, int D, int W>
+__global__ void __launch_bounds__(64 * W) pick_kernel(const SelectArgs a) {
+  __shared__ PickLds<W> lds;
+  __shared__ uint32_t keys[kLdsPages];
+  const int64_t unit = blockIdx.x;
+  const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
+  const int len = select_len(a, b);
+  const int pages = (len + a.page - 1) / a.page;
+  write_len(a, unit, len, pages);
+  if (pages <= a.keep) {
+    keep_all(a, unit, b, pages);
+    return;
+  }
+  clear(lds);
+  uint32_t* shared = a.keys + unit * unit_words(a.max_pages);
+  float scale = 0.0f;
+  for (int t = threadIdx.x; t < (pages + kTile - 1) / kTile; t += 64 * W) {
+    scale = fmaxf(scale, __builtin_bit_cast(float, shared[a.max_pages + t]));
+  }
+  if (pages <= kLdsPages) {
+    for (int p = threadIdx.x; p < pages; p += 64 * W) keys[p] = shared[p];
+    pick_pages<E, D, W>(a, lds, unit, b, h, pages, keys, scale);
+  } else {
+    pick_pages<E, D, W>(a, lds, unit, b, h, pages, shared, scale);
   }
 }
 
-// Whether one launch does both. A workgroup of it takes a sequence and KV head from
-// end to end, so it suits tables that its 16 waves cover in a few tiles each, and any
-// that fits when the units fill the device; otherwise the scores are spread over the
-// device first.
-constexpr int kOneLaunchPages = 2048;
-bool one_launch(int64_t units, int max_pages) {
-  return max_pages <= kOneLaunchPages || (max_pages <= kLdsPages && units >= current_cu_count());
+// Workgroups of a unit: as many as can have a tile for each of eight waves, within one
+// for each CU in all (a CU holds one or two, and the others wait for a round of their
+// own: 32 sequences of up to 1,024 pages 21 -> 28 us with four).
+int unit_workgroups(int64_t units, int max_pages) {
+  const int64_t most = cdiv(max_pages, kTile * 8);
+  const int64_t wanted = cdiv(static_cast<int64_t>(current_cu_count()), std::max<int64_t>(units, 1));
+  return static_cast<int>(std::max<int64_t>(1, std::min(most, wanted)));
 }
 
-template <typename E, int D>
-int launch_select(const SelectArgs& a, int64_t units, hipStream_t stream) {
-  if (one_launch(units, a.max_pages)) {
-    select_kernel<E, D><<<static_cast<unsigned>(units), kPickThreads, 0, stream>>>(a);
+// Whether a workgroup has 16 waves: where it has a unit to itself and more tiles than
+// eight waves take at once, and for long tables, whose keys one workgroup ranks. Measured
+// (us, 8 -> 16 waves): 32 sequences of up to 1,024 pages, 8 KV heads 21.2 -> 18.6, one
+// sequence of 8,192 29.0 -> 23.8; the other way one of 1,024 12.7 -> 11.4, of 128 8.4 ->
+// 7.6, and at head_dim 256, whose registers leave room for eight, 20 -> 13.3.
+bool wide_workgroups(int head_dim, int wgs, int max_pages) {
+  return head_dim <= 128 && ((wgs == 1 && max_pages > kTile * 8) || max_pages > 2048);
+}
+
+template <typename E, int D, int W>
+int launch_select(SelectArgs& a, int64_t units, int wgs, hipStream_t stream) {
+  a.arrivals = wgs > 1 && a.max_pages > a.keep && a.max_pages <= kLdsPages ? arrival_counters(units, stream) : nullptr;
+  if (a.arrivals != nullptr || (wgs == 1 && a.max_pages <= kLdsPages) || a.max_pages <= a.keep) {
+    const dim3 grid(static_cast<unsigned>(a.arrivals != nullptr ? wgs : 1), static_cast<unsigned>(units));
+    select_kernel<E, D, W><<<grid, 64 * W, 0, stream>>>(a);
     return check_launch("select_pages kernel launch");
   }
-  if (a.max_pages > a.keep) {  // else every page is kept
-    // About four tiles a wave.
-    const dim3 grid(static_cast<unsigned>(cdiv(a.max_pages, 16 * 4 * kScoreWaves)), static_cast<unsigned>(units));
-    score_kernel<E, D><<<grid, kScoreWaves * 64, 0, stream>>>(a);
-    const int st = check_launch("select_pages score kernel launch");
-    if (st != KL_OK) return st;
-  }
-  pick_kernel<E, D><<<static_cast<unsigned>(units), kPickThreads, 0, stream>>>(a);
+  const dim3 grid(static_cast<unsigned>(wgs), static_cast<unsigned>(units));
+  score_kernel<E, D, W><<<grid, 64 * W, 0, stream>>>(a);
+  const int st = check_launch("select_pages score kernel launch");
+  if (st != KL_OK) return st;
+  pick_kernel<E, D, W><<<static_cast<unsigned>(units), 64 * W, 0, stream>>>(a);
   return check_launch("select_pages kernel launch");
 }
 
 template <typename E>
-int dispatch_select(const SelectArgs& a, int dim, int64_t units, hipStream_t stream) {
-  return dim == 64    ? launch_select<E, 64>(a, units, stream)
-         : dim == 128 ? launch_select<E, 128>(a, units, stream)
-                      : launch_select<E, 256>(a, units, stream);
+int dispatch_select(SelectArgs& a, int dim, int64_t units, hipStream_t stream) {
+  const int wgs = unit_workgroups(units, a.max_pages);
+  const bool wide = wide_workgroups(dim, wgs, a.max_pages);
+  if (dim == 64) {
+    return wide ? launch_select<E, 64, 16>(a, units, wgs, stream) : launch_select<E, 64, 8>(a, units, wgs, stream);
+  }
+  if (dim == 128) {
+    return wide ? launch_select<E, 128, 16>(a, units, wgs, stream) : launch_select<E, 128, 8>(a, units, wgs, stream);
+  }
+  return launch_select<E, 256, 8>(a, units, wgs, stream);
 }
 
 bool head_dim_ok(int dim) { return dim == 64 || dim == 128 || dim == 256; }
@@ -997,7 +1075,9 @@ extern "C" int kl_select_pages_workspace(int batch, int num_kv_heads, int max_pa
   }
   const int64_t units = static_cast<int64_t>(batch) * num_kv_heads;
   if (out_workspace) {
-    *out_workspace = one_launch(units, max_pages) ? 0 : static_cast<size_t>(units) * static_cast<size_t>(max_pages) * 4;
+    *out_workspace = unit_workgroups(units, max_pages) == 1 && max_pages <= kLdsPages
+                         ? 0
+                         : static_cast<size_t>(units) * static_cast<size_t>(unit_words(max_pages)) * 4;
   }
   return ok();
 }

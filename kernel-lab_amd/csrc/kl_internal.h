@@ -23,6 +23,13 @@ int check_launch(const char* what);
 // Compute units of the current device (cached per device), or 0 on error.
 int current_cu_count();
 
+// Counters for a launch in which the last of a unit's workgroups finishes the unit:
+// `units` of them, zero when the launch starts and left zero by it. Only launches
+// ordered with this one share them (the stream's own, or those of its capture and
+// stream). Null where the library has none left, for more than 8,192 units, and on
+// hipStreamPerThread: the caller then takes a second launch.
+uint32_t* arrival_counters(int64_t units, hipStream_t stream);
+
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace kl

@@ -2868,6 +2868,14 @@ uint32_t* arrival_region(hipStream_t stream) {
   return remember(taken++);
 }
 
+}  // namespace
+
+uint32_t* arrival_counters(int64_t units, hipStream_t stream) {
+  return units <= kArrivalCounters ? arrival_region(stream) : nullptr;
+}
+
+namespace {
+
 // How the last decode launch on this thread combined split units
 // (kl_paged_decode_last_merge).
 thread_local int g_last_merge = KL_MERGE_NONE;

@@ -229,7 +229,7 @@ def test_through_c_abi(gpu_ops, pages):
     host = problem([16 * pages, 16 * 40 + 3], 16, 4, 128, torch.bfloat16, 16)
     q, edges, scale, table, lens = (t.cuda() for t in host)
     ws = ctypes.c_size_t(0)
-    assert lib.kl_select_pages_workspace(2, 4, pages, ctypes.byref(ws)) == 0 and ws.value == (0 if pages == 90 else 2 * 4 * pages * 4)
+    assert lib.kl_select_pages_workspace(2, 4, pages, ctypes.byref(ws)) == 0 and (ws.value == 0 if pages == 90 else ws.value >= 2 * 4 * pages * 4)
     work = torch.empty(max(1, ws.value), dtype=torch.uint8, device="cuda")
     out, out_lens = torch.empty(2, 4, 12, dtype=torch.int32, device="cuda"), torch.empty(2, 4, dtype=torch.int32, device="cuda")
 
