@@ -223,6 +223,15 @@ struct PageScaled : Fp8E4M3 {};
 template <typename KVF>
 constexpr bool kPageScaled = std::is_base_of_v<PageScaled, KVF>;
 
+// Cache policy of a segment's K/V loads. A head's row of 64 bytes is half a 128-byte
+// line whose other half is the next head's, so lines may stay for it: 32/8/64 B=64 of
+// 4,096 tokens 95 -> 90 us, up to 4,096 53 -> 46.5. (What bounds these is still the
+// number of 64-byte requests, as many as head_dim 128 makes of 128 bytes.)
+template <typename KVF, int D>
+constexpr int kLinePolicy() {
+  return kPageScaled<KVF> && D * KVF::kBytes < 128 ? 0 : kKvPolicy;
+}
+
 // Whether the softmax weights keep fp32's precision up to the P V products, as
 // the VALU kernel's do: fp32, and small pages, which are 16-bit caches whose
 // weights go in as three bf16 parts or two fp16 ones (2^-24 of a weight). A
@@ -845,7 +854,7 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
       const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<KS*>(cache + src), static_cast<short>(0),
                                                        live ? 0x7fffffff : 0, kBufferDword3);
 #pragma unroll
-      for (int c = 0; c < NL; ++c) f[c] = buffer_load16<kKvPolicy>(r, kv_off[c]);
+      for (int c = 0; c < NL; ++c) f[c] = buffer_load16<kLinePolicy<KVF, D>()>(r, kv_off[c]);
     }
   };
   auto load_block = [&](const auto& src, u32x4 (&kf)[NL], u32x4 (&vf)[NL], bool live) {
@@ -862,9 +871,9 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
       const auto vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<KS*>(vc + src), static_cast<short>(0), records,
                                                         kBufferDword3);
 #pragma unroll
-      for (int c = 0; c < NL; ++c) kf[c] = buffer_load16<kKvPolicy>(kr, kv_off[c]);
+      for (int c = 0; c < NL; ++c) kf[c] = buffer_load16<kLinePolicy<KVF, D>()>(kr, kv_off[c]);
 #pragma unroll
-      for (int c = 0; c < NL; ++c) vf[c] = buffer_load16<kKvPolicy>(vr, kv_off[c]);
+      for (int c = 0; c < NL; ++c) vf[c] = buffer_load16<kLinePolicy<KVF, D>()>(vr, kv_off[c]);
     }
   };
   // PageScaled: the loads of a block's scales, then its K and V, so that the wait
@@ -3408,6 +3417,14 @@ int decode_entry(kl_dtype dtype, Cache cache, void* out, const void* q, const vo
   }
   const Options opt = options();
   const bool use_mfma = kv8 || !opt.force_valu();
+  // Tables per KV head hold about as many pages each (kl_select_pages gives every one
+  // the same number at most), so a full batch takes one uniform split. Measured (us,
+  // balanced -> uniform, 32 query heads over 8): 32 sequences of 128 pages of 16 35.0 ->
+  // 28.2, 64 of 64 pages 35.2 -> 30.4.
+  if (cache == Cache::kPageScalesHeadTables && num_splits == 0 && opt.balance() < 0 &&
+      static_cast<int64_t>(batch) * cdiv(num_q_heads, mfma_heads_cap(num_q_heads, head_dim)) >= current_cu_count()) {
+    num_splits = 1;
+  }
   Plan p;
   int st = decode_plan(opt, dtype, batch, num_q_heads, num_kv_heads, head_dim, page_size, max_pages, num_splits,
                        current_cu_count(), use_mfma, &p);

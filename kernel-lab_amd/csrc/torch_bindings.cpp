@@ -26,7 +26,8 @@
 // of a model served in 8 bits: `rms_norm_fp8` and its two residual forms (FP8
 // output with scales), `append_kv_fp8` (new tokens into a cache with scales per
 // page and KV head), `paged_decode_attention_fp8_pages` over that cache, and
-// `select_pages` (the pages that sparse decode attends).
+// `select_pages` (the pages that sparse decode attends); `rms_norm_fp8_alloc` and
+// `fused_add_rms_norm_fp8_alloc` return the norms' outputs.
 //
 // Outputs are caller-allocated ("Tensor!" = mutated in place). The only
 // allocation here is the split-KV workspace, taken from PyTorch's caching
@@ -39,6 +40,7 @@
 
 #include <algorithm>
 #include <optional>
+#include <tuple>
 #include <vector>
 
 #include "kernel_lab.h"
@@ -192,6 +194,51 @@ void fused_add_rms_norm_fp8_new(at::Tensor& out, at::Tensor& scales, at::Tensor&
                                 const at::Tensor& residual, const at::Tensor& weight, double eps,
                                 int64_t scale_group) {
   rms_norm_fp8_impl(out, scales, x, &residual, &residual_out, weight, eps, scale_group);
+}
+
+// The same with outputs allocated here: three allocations from Python cost a small
+// call more than its kernel takes.
+struct Fp8Outputs {
+  at::Tensor out, scales;
+};
+
+Fp8Outputs empty_fp8(const at::Tensor& x, int64_t scale_group) {
+  TORCH_CHECK(x.dim() >= 1 && scale_group >= 0 && (scale_group == 0 || x.size(-1) % scale_group == 0),
+              "hidden must be a multiple of scale_group");
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = scale_group == 0 ? 1 : x.size(-1) / scale_group;
+  return {at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), at::empty(shape, x.options().dtype(at::kFloat))};
+}
+
+std::tuple<at::Tensor, at::Tensor> rms_norm_fp8_alloc(const at::Tensor& x, const at::Tensor& weight, double eps,
+                                                      int64_t scale_group) {
+  Fp8Outputs o = empty_fp8(x, scale_group);
+  rms_norm_fp8_impl(o.out, o.scales, x, nullptr, nullptr, weight, eps, scale_group);
+  return {o.out, o.scales};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> fused_add_rms_norm_fp8_alloc(const at::Tensor& x,
+                                                                            const at::Tensor& residual,
+                                                                            const at::Tensor& weight, double eps,
+                                                                            int64_t scale_group) {
+  Fp8Outputs o = empty_fp8(x, scale_group);
+  at::Tensor residual_out = at::empty(x.sizes(), x.options());
+  rms_norm_fp8_impl(o.out, o.scales, x, &residual, &residual_out, weight, eps, scale_group);
+  return {o.out, o.scales, residual_out};
+}
+
+// Shapes alone, for tracing.
+std::tuple<at::Tensor, at::Tensor> rms_norm_fp8_alloc_meta(const at::Tensor& x, const at::Tensor&, double,
+                                                           int64_t scale_group) {
+  Fp8Outputs o = empty_fp8(x, scale_group);
+  return {o.out, o.scales};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> fused_add_rms_norm_fp8_alloc_meta(const at::Tensor& x,
+                                                                                 const at::Tensor&, const at::Tensor&,
+                                                                                 double, int64_t scale_group) {
+  Fp8Outputs o = empty_fp8(x, scale_group);
+  return {o.out, o.scales, at::empty(x.sizes(), x.options())};
 }
 
 void rms_norm(at::Tensor& out, const at::Tensor& x, const at::Tensor& weight, double eps) {
@@ -594,6 +641,10 @@ TORCH_LIBRARY(kernel_lab, m) {
   m.def(
       "fused_add_rms_norm_fp8_new(Tensor! out, Tensor! scales, Tensor! residual_out, Tensor x, Tensor residual, "
       "Tensor weight, float eps, int scale_group=0) -> ()");
+  m.def("rms_norm_fp8_alloc(Tensor x, Tensor weight, float eps, int scale_group=0) -> (Tensor, Tensor)");
+  m.def(
+      "fused_add_rms_norm_fp8_alloc(Tensor x, Tensor residual, Tensor weight, float eps, int scale_group=0) "
+      "-> (Tensor, Tensor, Tensor)");
   m.def(
       "paged_decode_attention_fp8_pages(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, "
       "Tensor block_table, Tensor seq_lens, float scale, Tensor k_scale, Tensor v_scale, "
@@ -619,7 +670,15 @@ TORCH_LIBRARY_IMPL(kernel_lab, CUDA, m) {
   m.impl("rms_norm_fp8", &rms_norm_fp8);
   m.impl("fused_add_rms_norm_fp8", &fused_add_rms_norm_fp8);
   m.impl("fused_add_rms_norm_fp8_new", &fused_add_rms_norm_fp8_new);
+  m.impl("rms_norm_fp8_alloc", &rms_norm_fp8_alloc);
+  m.impl("fused_add_rms_norm_fp8_alloc", &fused_add_rms_norm_fp8_alloc);
   m.impl("paged_decode_attention_fp8_pages", &paged_decode_attention_fp8_pages);
   m.impl("append_kv_fp8", &append_kv_fp8);
   m.impl("select_pages", &select_pages);
+}
+
+// The operators that return their outputs; the others mutate what they are given.
+TORCH_LIBRARY_IMPL(kernel_lab, Meta, m) {
+  m.impl("rms_norm_fp8_alloc", &rms_norm_fp8_alloc_meta);
+  m.impl("fused_add_rms_norm_fp8_alloc", &fused_add_rms_norm_fp8_alloc_meta);
 }

@@ -117,17 +117,24 @@ def fused_add_rms_norm_(
 FP8_SCALE_GROUPS = (32, 64, 128, 256)
 
 
-def _fp8_outputs(x: torch.Tensor, group_size: int | None) -> tuple[torch.Tensor, torch.Tensor, int]:
-    """Empty codes and scales for x, and the operator's scale_group."""
-    hidden = x.shape[-1]
-    group = 0 if group_size is None or group_size == hidden else int(group_size)
-    if group and group not in FP8_SCALE_GROUPS:
+def _scale_group(hidden: int, group_size: int | None) -> int:
+    """The operators' scale_group: 0 for a scale per row."""
+    if group_size is None or group_size == hidden:
+        return 0
+    if group_size not in FP8_SCALE_GROUPS:
         raise ValueError(f"group_size must be None (a scale per row) or one of {FP8_SCALE_GROUPS}, got {group_size}")
-    if group and hidden % group:
-        raise ValueError(f"hidden size {hidden} is not a multiple of group_size {group}")
+    if hidden % group_size:
+        raise ValueError(f"hidden size {hidden} is not a multiple of group_size {group_size}")
+    return int(group_size)
+
+
+def _fp8_outputs(x: torch.Tensor, group: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Empty codes and scales for x."""
     out = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((*x.shape[:-1], hidden // group if group else 1), dtype=torch.float32, device=x.device)
-    return out, scales, group
+    scales = torch.empty(
+        (*x.shape[:-1], x.shape[-1] // group if group else 1), dtype=torch.float32, device=x.device
+    )
+    return out, scales
 
 
 def rms_norm_fp8(
@@ -144,9 +151,12 @@ def rms_norm_fp8(
     """
     _check_rms(x, weight, None)
     _native.require_ops()
-    x = _rows_view(x)
-    out, scales, group = _fp8_outputs(x, group_size)
-    torch.ops.kernel_lab.rms_norm_fp8(out, scales, x, weight.contiguous(), eps, group)
+    group = _scale_group(x.shape[-1], group_size)
+    x, weight = _rows_view(x), weight.contiguous()
+    if _carries_nothing(x) and _carries_nothing(weight):
+        return torch.ops.kernel_lab.rms_norm_fp8_alloc(x, weight, eps, group)
+    out, scales = _fp8_outputs(x, group)
+    torch.ops.kernel_lab.rms_norm_fp8(out, scales, x, weight, eps, group)
     return out, scales
 
 
@@ -157,17 +167,13 @@ def fused_add_rms_norm_fp8(
     (codes, scales, new_residual) and leaves ``residual`` untouched."""
     _check_rms(x, weight, residual)
     _native.require_ops()
-    x = _rows_view(x)
-    out, scales, group = _fp8_outputs(x, group_size)
-    residual = residual.contiguous()
-    if _carries_nothing(residual):
-        new_residual = torch.empty_like(residual)
-        torch.ops.kernel_lab.fused_add_rms_norm_fp8_new(
-            out, scales, new_residual, x, residual, weight.contiguous(), eps, group
-        )
-    else:
-        new_residual = residual.clone()
-        torch.ops.kernel_lab.fused_add_rms_norm_fp8(out, scales, x, new_residual, weight.contiguous(), eps, group)
+    group = _scale_group(x.shape[-1], group_size)
+    x, residual, weight = _rows_view(x), residual.contiguous(), weight.contiguous()
+    if _carries_nothing(residual) and _carries_nothing(x) and _carries_nothing(weight):
+        return torch.ops.kernel_lab.fused_add_rms_norm_fp8_alloc(x, residual, weight, eps, group)
+    out, scales = _fp8_outputs(x, group)
+    new_residual = residual.clone()
+    torch.ops.kernel_lab.fused_add_rms_norm_fp8(out, scales, x, new_residual, weight, eps, group)
     return out, scales, new_residual
 
 
@@ -182,8 +188,9 @@ def fused_add_rms_norm_fp8_(
     (codes, scales) of rmsnorm(residual) as ``rms_norm_fp8`` does."""
     _check_rms(x, weight, residual)
     _native.require_ops()
+    group = _scale_group(x.shape[-1], group_size)
     x = _rows_view(x)
-    out, scales, group = _fp8_outputs(x, group_size)
+    out, scales = _fp8_outputs(x, group)
     torch.ops.kernel_lab.fused_add_rms_norm_fp8(out, scales, x, residual, weight, eps, group)
     return out, scales
 

@@ -178,8 +178,36 @@ def test_empty_inputs(gpu_ops):
     assert out.shape == (0, 64) and scales.shape == (0, 2)
 
 
-def test_compiles_and_replays(gpu_ops):
-    """Under torch.compile(fullgraph=True), and captured into a graph whose inputs change between replays."""
+@pytest.mark.parametrize("group", [None, 128])
+def test_compiles(gpu_ops, group):
+    """Under torch.compile(fullgraph=True): the functional and the in-place forms."""
+    x, r, w = inputs((16, 1024), torch.bfloat16)
+
+    def step(x, r, w):
+        out, scales, new = gpu_ops.fused_add_rms_norm_fp8(x, r, w, group_size=group)
+        plain, plain_scales = gpu_ops.rms_norm_fp8(new, w, group_size=group)
+        return out, scales, new, plain, plain_scales
+
+    want = step(x, r, w)
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(x, r, w)
+    for g, ok in zip(got, want):
+        assert torch.equal(g.contiguous().view(torch.uint8), ok.contiguous().view(torch.uint8))
+
+
+def test_inputs_with_a_history(gpu_ops):
+    """Parameters and a residual in a graph give the same values; no gradient passes the codes."""
+    x, r, w = inputs((4, 256), torch.float32)
+    want = gpu_ops.fused_add_rms_norm_fp8(x, r, w)
+    leaf, weight = r.clone().requires_grad_(), torch.nn.Parameter(w)
+    out, scales, new = gpu_ops.fused_add_rms_norm_fp8(x, leaf * 1.0, weight)
+    assert torch.equal(out.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(scales, want[1])
+    assert torch.equal(new.detach(), want[2]) and not out.requires_grad and not scales.requires_grad
+    plain = gpu_ops.rms_norm_fp8(x, weight)
+    assert torch.equal(plain[0].view(torch.uint8), gpu_ops.rms_norm_fp8(x, w)[0].view(torch.uint8))
+
+
+def test_replays(gpu_ops):
+    """Captured into a graph whose inputs change between replays."""
     x, r, w = inputs((16, 1024), torch.float16)
     want = gpu_ops.fused_add_rms_norm_fp8(x, r, w, group_size=128)
     out = torch.empty(16, 1024, dtype=torch.float8_e4m3fn, device="cuda")
