@@ -428,6 +428,14 @@ __host__ __device__ __forceinline__ int64_t unit_words(int64_t max_pages) {
   return max_pages + (max_pages + kTile - 1) / kTile;
 }
 
+// The unit of a workgroup, by the grid's y and z, and the grid for `units`.
+constexpr int kUnitsY = 32768;
+__device__ __forceinline__ int64_t grid_unit() { return static_cast<int64_t>(blockIdx.z) * kUnitsY + blockIdx.y; }
+inline dim3 unit_grid(int wgs, int64_t units) {
+  return dim3(static_cast<unsigned>(wgs), static_cast<unsigned>(std::min<int64_t>(units, kUnitsY)),
+              static_cast<unsigned>(cdiv(units, kUnitsY)));
+}
+
 __device__ __forceinline__ int select_len(const SelectArgs& a, int b) {
   const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page;
   const int64_t len = as_constant(a.seq_lens)[b];
@@ -854,8 +862,9 @@ __global__ void __launch_bounds__(64 * W) select_kernel(const SelectArgs a) {
   __shared__ PickLds<W> lds;
   __shared__ uint32_t keys[kLdsPages];
   __shared__ int s_last;
-  const int64_t unit = blockIdx.y;
+  const int64_t unit = grid_unit();
   const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
+  if (b >= a.batch) return;
   const int len = select_len(a, b);
   const int pages = (len + a.page - 1) / a.page;
   const int tiles = (pages + kTile - 1) / kTile;
@@ -911,8 +920,9 @@ __global__ void __launch_bounds__(64 * W) select_kernel(const SelectArgs a) {
 // The same in two launches: for tables past kLdsPages, and where there are no counters.
 template <typename E, int D, int W>
 __global__ void __launch_bounds__(64 * W) score_kernel(const SelectArgs a) {
-  const int64_t unit = blockIdx.y;
+  const int64_t unit = grid_unit();
   const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
+  if (b >= a.batch) return;
   const int pages = (select_len(a, b) + a.page - 1) / a.page;
   if (pages <= a.keep) return;
   uint32_t* shared = a.keys + unit * unit_words(a.max_pages);
@@ -927,8 +937,9 @@ template <typename E, int D, int W>
 __global__ void __launch_bounds__(64 * W) pick_kernel(const SelectArgs a) {
   __shared__ PickLds<W> lds;
   __shared__ uint32_t keys[kLdsPages];
-  const int64_t unit = blockIdx.x;
+  const int64_t unit = grid_unit();
   const int b = static_cast<int>(unit / a.heads), h = static_cast<int>(unit % a.heads);
+  if (b >= a.batch) return;
   const int len = select_len(a, b);
   const int pages = (len + a.page - 1) / a.page;
   write_len(a, unit, len, pages);
@@ -972,15 +983,13 @@ template <typename E, int D, int W>
 int launch_select(SelectArgs& a, int64_t units, int wgs, hipStream_t stream) {
   a.arrivals = wgs > 1 && a.max_pages > a.keep && a.max_pages <= kLdsPages ? arrival_counters(units, stream) : nullptr;
   if (a.arrivals != nullptr || (wgs == 1 && a.max_pages <= kLdsPages) || a.max_pages <= a.keep) {
-    const dim3 grid(static_cast<unsigned>(a.arrivals != nullptr ? wgs : 1), static_cast<unsigned>(units));
-    select_kernel<E, D, W><<<grid, 64 * W, 0, stream>>>(a);
+    select_kernel<E, D, W><<<unit_grid(a.arrivals != nullptr ? wgs : 1, units), 64 * W, 0, stream>>>(a);
     return check_launch("select_pages kernel launch");
   }
-  const dim3 grid(static_cast<unsigned>(wgs), static_cast<unsigned>(units));
-  score_kernel<E, D, W><<<grid, 64 * W, 0, stream>>>(a);
+  score_kernel<E, D, W><<<unit_grid(wgs, units), 64 * W, 0, stream>>>(a);
   const int st = check_launch("select_pages score kernel launch");
   if (st != KL_OK) return st;
-  pick_kernel<E, D, W><<<static_cast<unsigned>(units), 64 * W, 0, stream>>>(a);
+  pick_kernel<E, D, W><<<unit_grid(1, units), 64 * W, 0, stream>>>(a);
   return check_launch("select_pages kernel launch");
 }
 
@@ -1105,9 +1114,9 @@ extern "C" int kl_select_pages(kl_dtype dtype, int32_t* out_table, int32_t* out_
     return fail(KL_ERR_INVALID_ARGUMENT, "first_pages >= 0 and last_pages >= 1 must fit num_selected");
   }
   const int64_t units = static_cast<int64_t>(batch) * num_kv_heads;
-  if (units > 65535 || static_cast<int64_t>(max_pages) * page_size > 0x7fffffffLL ||
+  if (units > 0x7fffffffLL || static_cast<int64_t>(max_pages) * page_size > 0x7fffffffLL ||
       static_cast<int64_t>(num_selected) * page_size > 0x7fffffffLL) {
-    return fail(KL_ERR_UNSUPPORTED, "more than 65535 (sequence, KV head) pairs, or tables past 2^31 tokens");
+    return fail(KL_ERR_UNSUPPORTED, "more than 2^31 (sequence, KV head) pairs, or tables past 2^31 tokens");
   }
   if (batch == 0) return ok();
   if (max_pages < 1) return fail(KL_ERR_INVALID_ARGUMENT, "max_pages must be >= 1");

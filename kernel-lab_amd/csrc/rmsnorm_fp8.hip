@@ -281,6 +281,12 @@ int launch_typed(uint8_t* out, float* scales, const typename E::S* x, typename E
   const int threads = static_cast<int>(
       std::min<int64_t>(kMaxThreads, std::max<int64_t>(64, cdiv(cdiv(packs, kPacksPerThread), 64) * 64)));
   const int npack = static_cast<int>(cdiv(packs, threads));
+  // A grid of 2^32 threads and more along x wraps without an error.
+  const bool narrow = hidden >= VEC && packs <= kRowsMaxPacks;
+  const int row_threads = !narrow ? kMaxThreads : packs <= 4 ? 4 : packs <= 8 ? 8 : packs <= 16 ? 16 : packs <= 32 ? 32 : 64;
+  if ((narrow ? rows : static_cast<int64_t>(gx)) * row_threads > 0xffffffffLL - kRowsThreads) {
+    return fail(KL_ERR_UNSUPPORTED, "too many rows for one launch");
+  }
   auto rows_kernel = [&](auto lanes, auto al) {
     constexpr int L = decltype(lanes)::value;
     norm8_rows_kernel<E, L, HAS_RES, decltype(al)::value>

@@ -152,6 +152,7 @@ void rms_norm_fp8_impl(at::Tensor& out, at::Tensor& scales, const at::Tensor& x,
   }
   TORCH_CHECK(x.dim() >= 1 && (x.stride(-1) == 1 || x.size(-1) <= 1), "x must have a contiguous last dimension");
   const int64_t hidden = x.size(-1);
+  TORCH_CHECK(hidden > 0, "a row needs at least one element");
   TORCH_CHECK(weight.scalar_type() == x.scalar_type() && weight.is_contiguous() && weight.dim() == 1 &&
                   weight.numel() == hidden,
               "weight needs one contiguous value of x's dtype per hidden element (", weight.numel(), " values, hidden ",

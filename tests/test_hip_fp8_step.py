@@ -88,3 +88,39 @@ def test_a_few_tokens(gpu_ops, dtype, captured):
         close(sparse, *ref.decode(q, *cache, *want, host["k_scale"], host["v_scale"]), dtype)
         close(full, *ref.decode(q, *cache, host["block_table"], lens, host["k_scale"], host["v_scale"]), dtype)
         assert float(full[2].abs().max()) == 0.0 and float(sparse[2].abs().max()) == 0.0
+
+
+def test_compiled_and_on_a_stream_of_its_own(gpu_ops):
+    """append, selection and both decodes under torch.compile(fullgraph=True), on a side stream."""
+    batch, dtype = 3, torch.bfloat16
+    dev, host = make([60, 40, 17], HKV, D, PAGE)
+    lens = torch.tensor([50, 33, 16], dtype=torch.int32)
+    k, v = torch.randn(2, batch, HKV, D, generator=torch.Generator().manual_seed(1)).to(dtype)
+    q = torch.randn(batch, HQ, D, generator=torch.Generator().manual_seed(2)).to(dtype)
+    full = torch.randn(2, 99, HKV, D, generator=torch.Generator().manual_seed(3)).to(dtype)
+    off = torch.tensor([0, 50, 83, 99], dtype=torch.int32)
+    gpu_ops.append_kv_fp8(full[0].cuda(), full[1].cuda(), dev["k"], dev["v"], dev["k_scale"], dev["v_scale"], dev["block_table"],
+                          lens.cuda(), new_offsets=off.cuda(), k_bounds=dev["bounds"])
+    ref.append(full[0], full[1], host, lens, off)
+
+    def step(q, k, v, kc, vc, ks, vs, bounds, table, lens):
+        gpu_ops.append_kv_fp8(k, v, kc, vc, ks, vs, table, lens, k_bounds=bounds)
+        pages, some = gpu_ops.select_pages(q, bounds, ks, table, lens, 2, PAGE)
+        return (pages, some, gpu_ops.paged_decode_attention(q, kc, vc, pages, some, k_scale=ks, v_scale=vs),
+                gpu_ops.paged_decode_attention(q, kc, vc, table, lens, k_scale=ks, v_scale=vs))
+
+    compiled = torch.compile(step, fullgraph=True, backend="aot_eager")
+    lens = lens + 1
+    args = [t.cuda() for t in (q, k, v)] + [dev[n] for n in ("k", "v", "k_scale", "v_scale", "bounds", "block_table")] + [lens.cuda()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        pages, some, sparse, dense = compiled(*args)
+    torch.cuda.synchronize()
+    ref.append(k, v, host, lens)
+    same(dev, host)
+    want = ref.select(q, dev["bounds"].cpu(), host["k_scale"], host["block_table"], lens, 2, PAGE)
+    assert torch.equal(pages.cpu(), want[0]) and torch.equal(some.cpu(), want[1])
+    cache = dev["k"].cpu(), dev["v"].cpu()
+    close(sparse, *ref.decode(q, *cache, *want, host["k_scale"], host["v_scale"]), dtype)
+    close(dense, *ref.decode(q, *cache, host["block_table"], lens, host["k_scale"], host["v_scale"]), dtype)

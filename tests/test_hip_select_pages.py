@@ -179,6 +179,62 @@ def test_many_rows(gpu_ops):
     check(gpu_ops, *problem(lens, 32, 8, 64, torch.float16, 32), 16, 32, first=1, last=2)
 
 
+def test_more_rows_than_a_grid_dimension(gpu_ops):
+    """40,000 sequences, (sequence, KV head) pairs past the grid's second dimension."""
+    batch, page, width = 40000, 16, 6
+    g = torch.Generator().manual_seed(0)
+    edges = torch.randn(50, 2, 2, 64, generator=g).mul(50).sort(2).values.to(F8)
+    scale = 0.01 + torch.rand(50, 2, generator=g)
+    table = torch.randint(0, 50, (batch, width), generator=g, dtype=torch.int32)
+    lens = torch.randint(0, page * width + 1, (batch,), generator=g, dtype=torch.int32)
+    q = torch.randn(batch, 4, 64, generator=g).to(torch.bfloat16)
+    got = gpu_ops.select_pages(*(t.cuda() for t in (q, edges, scale, table, lens)), 3, page)
+    rows = torch.tensor([0, 1, 16383, 16384, 20000, 32767, 32768, 39999])
+    want = ref.select(q[rows], edges, scale, table[rows], lens[rows], 3, page)
+    assert torch.equal(got[0].cpu()[rows], want[0]) and torch.equal(got[1].cpu()[rows], want[1])
+
+
+def test_two_streams_at_once(gpu_ops):
+    """Tables whose scores several workgroups share, on two streams: each has counters of its own."""
+    args = [tuple(t.cuda() for t in problem([16 * 900, 16 * 500], 8, 2, 128, torch.bfloat16, 16, seed=s)) for s in range(2)]
+    want = [gpu_ops.select_pages(*a, 40, 16) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(gpu_ops.select_pages(*args[i], 40, 16))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for table, lens in got[i]:
+            assert torch.equal(table, want[i][0]) and torch.equal(lens, want[i][1])
+
+
+def test_two_captured_graphs_at_once(gpu_ops):
+    """Two graphs captured one after the other and replayed on two streams together."""
+    args = [tuple(t.cuda() for t in problem([16 * 900, 16 * 500], 8, 2, 128, torch.float16, 16, seed=s)) for s in range(2)]
+    want = [gpu_ops.select_pages(*a, 40, 16) for a in args]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for a in args:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(gpu_ops.select_pages(*a, 40, 16))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for t, n in got:
+            t.zero_()
+            n.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(got[i][0], want[i][0]) and torch.equal(got[i][1], want[i][1])
+
+
 def test_empty_batch(gpu_ops):
     q, edges, scale, table, lens = problem([16], 8, 2, 64, torch.bfloat16, 16)
     got = gpu_ops.select_pages(q[:0].cuda(), edges.cuda(), scale.cuda(), table[:0].cuda(), lens[:0].cuda(), 8, 16)
