@@ -108,12 +108,8 @@ __device__ __forceinline__ void norm8_row(uint8_t* out, float* scales, const typ
     a[k] = load_at<ALIGNED, P>(x, off[k]);
     if constexpr (HAS_RES) b[k] = load_at<ALIGNED, P>(res, off[k]);
   }
-  // Beside eight packs of x and the residual the weights would spill.
-  constexpr bool kEarlyWeights = NPACK <= 4;
-  if constexpr (kEarlyWeights) {
 #pragma unroll
-    for (int k = 0; k < NPACK; ++k) w[k] = load_at<ALIGNED, P>(weight, off[k]);
-  }
+  for (int k = 0; k < NPACK; ++k) w[k] = load_at<ALIGNED, P>(weight, off[k]);
   float sum_sq = 0.0f;
 #pragma unroll
   for (int k = 0; k < NPACK; ++k) {
@@ -133,10 +129,6 @@ __device__ __forceinline__ void norm8_row(uint8_t* out, float* scales, const typ
     }
   };
   if constexpr (HAS_RES && ALIGNED) store_residual();
-  if constexpr (!kEarlyWeights) {
-#pragma unroll
-    for (int k = 0; k < NPACK; ++k) w[k] = load_at<ALIGNED, P>(weight, off[k]);
-  }
   // x w: every scale and code comes from it.
   float p[NPACK][VEC];
   float most = 0.0f;
@@ -205,9 +197,10 @@ __global__ void __launch_bounds__(kRowsThreads)
       });
 }
 
-// Rows of less than a pack, and rows past the registers of a workgroup (more than 8
-// packs per thread, 4 unaligned), element by element: the squares (writing the
-// new residual), then each group's largest |y|, then its codes, all read again
+// Rows of less than a pack, and rows past the registers of a workgroup (more than 4
+// packs per thread: 32,768 elements of 16 bits, 16,384 of fp32; eight packs, their
+// products and the weights would spill), element by element: the squares (writing
+// the new residual), then each group's largest |y|, then its codes, all read again
 // from memory.
 template <typename E, bool HAS_RES>
 __global__ void __launch_bounds__(kMaxThreads)
@@ -263,6 +256,7 @@ template <int N>
 using IntC = std::integral_constant<int, N>;
 
 constexpr int kRowsMaxPacks = 64;   // widest row of norm8_rows_kernel: a pack per lane of a wave
+constexpr int kMaxPacks = 4;        // per thread of norm8_kernel
 constexpr int kPacksPerThread = 2;  // aimed at beyond (rmsnorm.hip has the measurements)
 
 template <typename E, bool HAS_RES>
@@ -310,13 +304,11 @@ int launch_typed(uint8_t* out, float* scales, const typename E::S* x, typename E
       rows_kernel(IntC<64>{}, al);
     } else if (npack <= 2) {
       wide_kernel(IntC<2>{}, al);
-    } else if (npack <= 4) {
-      wide_kernel(IntC<4>{}, al);
-    } else if constexpr (decltype(al)::value) {
-      wide_kernel(IntC<8>{}, al);
+    } else {
+      wide_kernel(IntC<kMaxPacks>{}, al);
     }
   };
-  if (hidden < VEC || npack > (aligned ? 8 : 4)) {
+  if (hidden < VEC || npack > kMaxPacks) {
     norm8_loop_kernel<E, HAS_RES><<<grid, hidden < VEC ? 64 : kMaxThreads, 0, stream>>>(
         out, scales, x, res, res_out, w, hidden, group, xm, eps);
   } else if (aligned) {
