@@ -26,8 +26,8 @@
 // of a model served in 8 bits: `rms_norm_fp8` and its two residual forms (FP8
 // output with scales), `append_kv_fp8` (new tokens into a cache with scales per
 // page and KV head), `paged_decode_attention_fp8_pages` over that cache, and
-// `select_pages` (the pages that sparse decode attends); `rms_norm_fp8_alloc` and
-// `fused_add_rms_norm_fp8_alloc` return the norms' outputs.
+// `select_pages` (the pages that sparse decode attends); the operators
+// named `..._alloc` return their outputs.
 //
 // Outputs are caller-allocated ("Tensor!" = mutated in place). The only
 // allocation here is the split-KV workspace, taken from PyTorch's caching
@@ -470,6 +470,23 @@ void paged_decode_attention_fp8_pages(at::Tensor& out, const at::Tensor& q, cons
       "paged_decode_attention_fp8_pages");
 }
 
+// The same with the output allocated here (see rms_norm_fp8_alloc).
+at::Tensor paged_decode_attention_fp8_pages_alloc(const at::Tensor& q, const at::Tensor& k_cache,
+                                                  const at::Tensor& v_cache, const at::Tensor& block_table,
+                                                  const at::Tensor& seq_lens, double scale, const at::Tensor& k_scale,
+                                                  const at::Tensor& v_scale, int64_t num_splits, int64_t max_seq_len) {
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  paged_decode_attention_fp8_pages(out, q, k_cache, v_cache, block_table, seq_lens, scale, k_scale, v_scale, num_splits,
+                                   max_seq_len);
+  return out;
+}
+
+at::Tensor paged_decode_attention_fp8_pages_alloc_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
+                                                       const at::Tensor&, const at::Tensor&, double, const at::Tensor&,
+                                                       const at::Tensor&, int64_t, int64_t) {
+  return at::empty(q.sizes(), q.options());
+}
+
 // New tokens into the cache. k and v [tokens, kv heads, head_dim] may be strided
 // in their first two dimensions.
 void append_kv_fp8(const at::Tensor& k, const at::Tensor& v, at::Tensor& k_cache, at::Tensor& v_cache,
@@ -552,6 +569,30 @@ void select_pages(at::Tensor& out_table, at::Tensor& out_lens, const at::Tensor&
                       checked_int(keep, "num_selected"), checked_int(first_pages, "first_pages"),
                       checked_int(last_pages, "last_pages"), ws_bytes > 0 ? workspace.data_ptr() : nullptr, ws_bytes, current_stream(dev)),
       "select_pages");
+}
+
+// The same with the table and lengths allocated here.
+std::tuple<at::Tensor, at::Tensor> empty_selection(const at::Tensor& q, const at::Tensor& k_bounds, int64_t num_pages) {
+  TORCH_CHECK(q.dim() == 3 && k_bounds.dim() == 4 && num_pages >= 1,
+              "q is [batch, heads, dim], k_bounds [num_pages, num_kv_heads, 2, head_dim], num_pages at least 1");
+  const auto ints = q.options().dtype(at::kInt);
+  return {at::empty({q.size(0), k_bounds.size(1), num_pages}, ints), at::empty({q.size(0), k_bounds.size(1)}, ints)};
+}
+
+std::tuple<at::Tensor, at::Tensor> select_pages_alloc(const at::Tensor& q, const at::Tensor& k_bounds,
+                                                      const at::Tensor& k_scale, const at::Tensor& block_table,
+                                                      const at::Tensor& seq_lens, int64_t num_pages, int64_t page_size,
+                                                      int64_t first_pages, int64_t last_pages) {
+  auto out = empty_selection(q, k_bounds, num_pages);
+  select_pages(std::get<0>(out), std::get<1>(out), q, k_bounds, k_scale, block_table, seq_lens, page_size, first_pages,
+               last_pages);
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> select_pages_alloc_meta(const at::Tensor& q, const at::Tensor& k_bounds,
+                                                           const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                           int64_t num_pages, int64_t, int64_t, int64_t) {
+  return empty_selection(q, k_bounds, num_pages);
 }
 
 // Shared-prefix decode: attention over prefix tokens, then each sequence's own.
@@ -656,6 +697,13 @@ TORCH_LIBRARY(kernel_lab, m) {
   m.def(
       "select_pages(Tensor! out_table, Tensor! out_lens, Tensor q, Tensor k_bounds, Tensor k_scale, "
       "Tensor block_table, Tensor seq_lens, int page_size, int first_pages=1, int last_pages=1) -> ()");
+  m.def(
+      "paged_decode_attention_fp8_pages_alloc(Tensor q, Tensor k_cache, Tensor v_cache, "
+      "Tensor block_table, Tensor seq_lens, float scale, Tensor k_scale, Tensor v_scale, "
+      "int num_splits=0, int max_seq_len=0) -> Tensor");
+  m.def(
+      "select_pages_alloc(Tensor q, Tensor k_bounds, Tensor k_scale, Tensor block_table, Tensor seq_lens, "
+      "int num_pages, int page_size, int first_pages=1, int last_pages=1) -> (Tensor, Tensor)");
 }
 
 // ROCm tensors carry PyTorch's CUDA dispatch key.
@@ -676,10 +724,14 @@ TORCH_LIBRARY_IMPL(kernel_lab, CUDA, m) {
   m.impl("paged_decode_attention_fp8_pages", &paged_decode_attention_fp8_pages);
   m.impl("append_kv_fp8", &append_kv_fp8);
   m.impl("select_pages", &select_pages);
+  m.impl("paged_decode_attention_fp8_pages_alloc", &paged_decode_attention_fp8_pages_alloc);
+  m.impl("select_pages_alloc", &select_pages_alloc);
 }
 
 // The operators that return their outputs; the others mutate what they are given.
 TORCH_LIBRARY_IMPL(kernel_lab, Meta, m) {
   m.impl("rms_norm_fp8_alloc", &rms_norm_fp8_alloc_meta);
   m.impl("fused_add_rms_norm_fp8_alloc", &fused_add_rms_norm_fp8_alloc_meta);
+  m.impl("paged_decode_attention_fp8_pages_alloc", &paged_decode_attention_fp8_pages_alloc_meta);
+  m.impl("select_pages_alloc", &select_pages_alloc_meta);
 }

@@ -247,6 +247,10 @@ def paged_decode_attention(
     length for each (sequence, KV head): sparse decode over the pages that
     ``select_pages`` chose.
     """
+    if k_cache.dtype == torch.float8_e4m3fn and (block_table.dim() == 3 or _page_scales(k_scale, k_cache)):
+        return _decode_fp8_pages(
+            q, k_cache, v_cache, block_table, seq_lens, scale, num_splits, max_seq_len, out, k_scale, v_scale
+        )
     _check_decode(q, k_cache, v_cache)
     _native.require_ops()
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
@@ -257,17 +261,6 @@ def paged_decode_attention(
         if k_scale is None or v_scale is None:
             raise ValueError("an FP8 cache needs k_scale and v_scale")
         hkv = k_cache.shape[2]
-        # One page's [1, num_kv_heads] scales are scales per head.
-        if block_table.dim() == 3 or (k_cache.shape[0] > 1 and _page_scales(k_scale, k_cache)):
-            if not (_page_scales(k_scale, k_cache) and _page_scales(v_scale, k_cache)):
-                raise ValueError("k_scale and v_scale must both be [num_pages, num_kv_heads]")
-            if block_table.dim() == 3:
-                block_table, seq_lens = block_table.contiguous(), seq_lens.contiguous()
-            torch.ops.kernel_lab.paged_decode_attention_fp8_pages(
-                out, q, k_cache, v_cache, block_table, seq_lens, scale, k_scale, v_scale, int(num_splits or 0),
-                int(max_seq_len or 0),
-            )
-            return out
         ks = _head_scales(k_scale, hkv, q.device)
         vs = _head_scales(v_scale, hkv, q.device)
         torch.ops.kernel_lab.paged_decode_attention_fp8(
@@ -320,8 +313,35 @@ def cascade_decode_attention(
     return out
 
 
-def _page_scales(s: torch.Tensor | float, cache: torch.Tensor) -> bool:
-    return isinstance(s, torch.Tensor) and s.dim() == 2 and s.shape == (cache.shape[0], cache.shape[2])
+def _page_scales(s: torch.Tensor | float | None, cache: torch.Tensor) -> bool:
+    """Whether s is [num_pages, num_kv_heads]. (One page's [1, num_kv_heads] are scales per head as well.)"""
+    return isinstance(s, torch.Tensor) and s.dim() == 2 and s.shape[0] > 1 and s.shape == (cache.shape[0], cache.shape[2])
+
+
+def _decode_fp8_pages(
+    q, k_cache, v_cache, block_table, seq_lens, scale, num_splits, max_seq_len, out, k_scale, v_scale
+) -> torch.Tensor:
+    """paged_decode_attention with scales per page and KV head; the operator checks the arguments."""
+    _native.require_ops()
+    if not (isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)):
+        raise ValueError("k_scale and v_scale must both be [num_pages, num_kv_heads]")
+    if k_scale.shape != v_scale.shape or k_scale.dim() != 2:
+        raise ValueError("k_scale and v_scale must both be [num_pages, num_kv_heads]")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    q = q.contiguous()
+    if block_table.dim() == 3:
+        block_table, seq_lens = block_table.contiguous(), seq_lens.contiguous()
+    splits, longest = int(num_splits or 0), int(max_seq_len or 0)
+    if out is None and _carries_nothing(q):
+        return torch.ops.kernel_lab.paged_decode_attention_fp8_pages_alloc(
+            q, k_cache, v_cache, block_table, seq_lens, scale, k_scale, v_scale, splits, longest
+        )
+    if out is None:
+        out = torch.empty_like(q)
+    torch.ops.kernel_lab.paged_decode_attention_fp8_pages(
+        out, q, k_cache, v_cache, block_table, seq_lens, scale, k_scale, v_scale, splits, longest
+    )
+    return out
 
 
 def append_kv_fp8(
@@ -361,12 +381,6 @@ def append_kv_fp8(
     no gradient passes through it.
     """
     _native.require_ops()
-    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
-        raise ValueError("k and v are [tokens, kv_heads, head_dim] and the caches [pages, page_size, kv_heads, head_dim]")
-    if k.shape[1:] != k_cache.shape[2:]:
-        raise ValueError(f"k is {tuple(k.shape)} but the cache has heads {tuple(k_cache.shape[2:])}")
-    if new_offsets is None and k.shape[0] != seq_lens.shape[0]:
-        raise ValueError("without new_offsets, k and v have one token per sequence")
     torch.ops.kernel_lab.append_kv_fp8(
         _rows_view(k), _rows_view(v), k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, new_offsets, k_bounds
     )
@@ -406,11 +420,15 @@ def select_pages(
         raise ValueError("num_q_heads must be a multiple of num_kv_heads")
     if first_pages < 0 or last_pages < 1 or first_pages + last_pages > num_pages:
         raise ValueError("first_pages >= 0 and last_pages >= 1 must fit num_pages")
+    q = q.contiguous()
+    if _carries_nothing(q):
+        return torch.ops.kernel_lab.select_pages_alloc(
+            q, k_bounds, k_scale, block_table, seq_lens, num_pages, page_size, first_pages, last_pages
+        )
     table = torch.empty((q.shape[0], num_kv_heads, num_pages), dtype=torch.int32, device=q.device)
     lens = torch.empty((q.shape[0], num_kv_heads), dtype=torch.int32, device=q.device)
     torch.ops.kernel_lab.select_pages(
-        table, lens, q.contiguous(), k_bounds, k_scale, block_table, seq_lens, int(page_size), int(first_pages),
-        int(last_pages),
+        table, lens, q, k_bounds, k_scale, block_table, seq_lens, page_size, first_pages, last_pages
     )
     return table, lens
 

@@ -202,6 +202,12 @@ def test_refusals(gpu_ops):
     lists = c.block_table[:, None].repeat(1, 2, 1), c.seq_lens[:, None].repeat(1, 2)
     with pytest.raises(ValueError, match="num_pages"):
         call(ks=c.k_scale[0], vs=c.v_scale[0], bt=lists[0], sl=lists[1])
+    with pytest.raises(ValueError, match="num_pages"):
+        call(ks=0.5, vs=0.5, bt=lists[0], sl=lists[1])
+    with pytest.raises(RuntimeError, match="k_scale"):
+        call(ks=c.k_scale[:-1], vs=c.v_scale[:-1], bt=lists[0], sl=lists[1])
+    with pytest.raises(RuntimeError, match="v_cache"):
+        gpu_ops.paged_decode_attention(q.cuda(), c.k_cache, c.v_cache[:-1], c.block_table, c.seq_lens, k_scale=c.k_scale, v_scale=c.v_scale)
     with pytest.raises(RuntimeError, match="per KV head"):
         call(bt=lists[0], sl=c.seq_lens)
     with pytest.raises(RuntimeError, match="per KV head"):
@@ -212,6 +218,23 @@ def test_refusals(gpu_ops):
     q8, kv8 = problem([20], 8, 2, 64, torch.float16, page=8)
     with pytest.raises(RuntimeError, match="multiple of 16"):
         run(gpu_ops, q8, kv8)
+
+
+def test_a_query_with_a_history_and_a_given_output(gpu_ops):
+    q, kv = problem([20, 40], 8, 2, 64, torch.float16)
+    c = on_gpu(kv)
+    args = c.k_cache, c.v_cache, c.block_table, c.seq_lens
+    want = gpu_ops.paged_decode_attention(q.cuda(), *args, k_scale=c.k_scale, v_scale=c.v_scale)
+    leaf = q.cuda().requires_grad_()
+    got = gpu_ops.paged_decode_attention(leaf, *args, k_scale=c.k_scale, v_scale=c.v_scale)
+    assert torch.equal(got, want) and not got.requires_grad
+    out = torch.empty_like(want)
+    assert gpu_ops.paged_decode_attention(q.cuda(), *args, k_scale=c.k_scale, v_scale=c.v_scale, out=out) is out
+    assert torch.equal(out, want)
+    every = torch.full((2,), 2, dtype=torch.int32)
+    table, lens = gpu_ops.select_pages(leaf, c.k_bounds, c.k_scale, c.block_table, c.seq_lens, 2, 16)
+    again = gpu_ops.select_pages(leaf.detach(), c.k_bounds, c.k_scale, c.block_table, c.seq_lens, 2, 16)
+    assert torch.equal(table, again[0]) and torch.equal(lens, again[1]) and table.shape == (2, 2, int(every[0]))
 
 
 @pytest.mark.parametrize("lists", [False, True])
