@@ -286,7 +286,8 @@ int kl_paged_decode_attention_fp8(kl_dtype dtype, void* out, const void* q,
  * as kl_select_pages writes them; size the workspace with kl_paged_decode_plan
  * for batch * num_kv_heads sequences of num_q_heads / num_kv_heads query heads and
  * one KV head. Other arguments, refusals and results as
- * kl_paged_decode_attention_fp8; a length of 0 gives zeros.
+ * kl_paged_decode_attention_fp8; a length of 0 gives zeros. The sums are fp32
+ * before they are normalised, so v_scale * decode(v) should stay below 2^96.
  */
 int kl_paged_decode_attention_fp8_pages(kl_dtype dtype, void* out, const void* q, const void* k_cache,
                                         const void* v_cache, const float* k_scale, const float* v_scale,
@@ -314,7 +315,9 @@ int kl_paged_decode_attention_fp8_pages(kl_dtype dtype, void* out, const void* q
  * new; one that holds earlier tokens takes max(old scale, new), and where that is
  * larger its codes c become e4m3((decode(c) * old) / scale). The new codes are
  * e4m3(x / scale), rounded to nearest even; a value that is not finite becomes a
- * NaN code, which no bound takes in. Slots behind the last token are not written.
+ * NaN code, which no bound takes in (a dimension without a finite key has the bounds
+ * 448 and -448). Slots behind the last token are not written. The caches and k_bounds
+ * are 16-byte aligned.
  *
  * Left alone, and nothing of theirs written: sequences whose length is less than
  * their new tokens (a padded batch gives them length 0) and whose offsets are not
@@ -336,9 +339,11 @@ int kl_append_kv_fp8(kl_dtype dtype, void* k_cache, void* v_cache, float* k_scal
  * over the tables it writes. No counterpart in the reference.
  *
  *   score = f32(k_scale * max over the KV head's query heads of
- *               sum_d max(q_d * lo_d, q_d * hi_d))
+ *               sum_d (min(q_d, 0) * lo_d + max(q_d, 0) * hi_d))
  * with lo and hi the decoded codes of k_bounds: no key of the page has a larger
- * q.k. The sums are formed in 64 bits. A NaN score counts as the largest finite one.
+ * q.k. (A dimension without a finite key, lo 448 and hi -448, lowers the score: its
+ * keys' q.k are NaN.) The sums are formed in 64 bits. A NaN score counts as the
+ * largest finite one. Scales are not negative.
  * The first `first_pages` pages of a sequence and its last `last_pages` come
  * before all others; of the rest the largest scores are kept, equal ones lowest
  * page first, num_selected pages in all, or every page of a shorter sequence.
@@ -349,7 +354,8 @@ int kl_append_kv_fp8(kl_dtype dtype, void* k_cache, void* v_cache, float* k_scal
  *   workspace  at least kl_select_pages_workspace's bytes (host arithmetic)
  *
  * q [batch, num_q_heads, head_dim] fp16 or bf16; head_dim 64, 128 or 256; first_pages
- * >= 0, last_pages >= 1, first_pages + last_pages <= num_selected.
+ * >= 0, last_pages >= 1, first_pages + last_pages <= num_selected; k_bounds 16-byte
+ * aligned.
  */
 int kl_select_pages_workspace(int batch, int num_kv_heads, int max_pages, size_t* out_workspace);
 

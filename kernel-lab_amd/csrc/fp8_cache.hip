@@ -390,8 +390,7 @@ int launch_append(AppendArgs& a, int64_t tiles, hipStream_t stream) {
 //
 // The largest q.k that a key within the page's bounds can have, for the query
 // head of the KV head's group where it is largest:
-//   score = f32(k_scale * max_g sum_d max(q_gd lo_d, q_gd hi_d))
-//         = f32(k_scale * max_g [lo hi] . [min(q_g, 0) max(q_g, 0)])
+//   score = f32(k_scale * max_g [lo hi] . [min(q_g, 0) max(q_g, 0)])
 // The sum is one of 64 bits, where it is exact for queries whose values span less
 // than about 2^30 (a product has 15 bits at most), so the order of its terms does
 // not decide which of two near scores is larger. In 64 bits for every page, the
@@ -498,7 +497,7 @@ struct ScoreQueries {
     for (int c = 0; c < C / 2; ++c) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const u32x4 w = g < a.group ? *reinterpret_cast<const u32x4*>(q + 64 * c + 8 * half) : u32x4{0, 0, 0, 0};
+        const u32x4 w = g < a.group ? load_at<false, u32x4>(q, 64 * c + 8 * half) : u32x4{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           // 0xffff in the halves that are negative (a NaN of either sign reaches one side).

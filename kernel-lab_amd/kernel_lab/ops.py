@@ -400,8 +400,8 @@ def select_pages(
     """Chooses the pages that each (sequence, KV head) attends: (table, lens).
 
     A page's score is k_scale * max over the KV head's query heads of
-    sum_d max(q_d lo_d, q_d hi_d), with lo and hi from ``k_bounds``: no key of
-    the page has a larger q.k. It is summed in 64 bits and rounded to float32;
+    sum_d min(q_d, 0) lo_d + max(q_d, 0) hi_d, with lo and hi from ``k_bounds``:
+    no key of the page has a larger q.k. It is summed in 64 bits and rounded to float32;
     a NaN counts as the largest finite score. The sequence's first
     ``first_pages`` and last ``last_pages`` (at least one) pages are kept in any
     case, then those of the largest scores, equal ones lowest page first, up to

@@ -141,7 +141,7 @@ def select(q, bounds, k_scale, block_table, seq_lens, num_pages, page, first=1, 
             score = torch.full((count,), float("-inf"), dtype=torch.float64)
             for g in range(h * group, (h + 1) * group):
                 x = q[b, g].double()
-                score = torch.maximum(score, torch.maximum(x * lo, x * hi).sum(-1))
+                score = torch.maximum(score, (x.clamp(max=0) * lo + x.clamp(min=0) * hi).sum(-1))
             score = (score * k_scale[ids, h].double()).float()
             most = torch.finfo(torch.float32).max
             score = score.nan_to_num(nan=most, posinf=most, neginf=float("-inf"))

@@ -104,6 +104,29 @@ def test_scores_that_are_not_numbers(gpu_ops):
     check(gpu_ops, q, edges, scale, table, lens, 6, 16)
 
 
+def test_dimensions_without_a_finite_key(gpu_ops):
+    """Their bounds are 448 and -448, and lower the score."""
+    q, edges, scale, table, lens = problem([16 * 64, 16 * 70], 8, 2, 64, torch.float16, 16, seed=9)
+    for b, p in ((0, 3), (0, 21), (1, 5), (1, 40)):
+        edges[table[b, p].long(), :, 0, 7] = 448.0
+        edges[table[b, p].long(), :, 1, 7] = -448.0
+    check(gpu_ops, q, edges, scale, table, lens, 30, 16)
+    flat = edges[table[0, 0].long()].expand_as(edges).clone()  # equal scores but for one page's
+    flat[table[0, 3].long(), :, 0, 7], flat[table[0, 3].long(), :, 1, 7] = 448.0, -448.0
+    got, _ = check(gpu_ops, q, flat, torch.ones_like(scale), table, lens, 63, 16)
+    assert not (got[0] == table[0, 3].item()).any()
+
+
+def test_a_query_at_any_address(gpu_ops):
+    q, edges, scale, table, lens = problem([16 * 64, 16 * 70], 8, 2, 64, torch.float16, 16, seed=9)
+    store = torch.empty(q.numel() + 1, dtype=q.dtype, device="cuda")
+    shifted = store[1:].view(q.shape)
+    shifted.copy_(q)
+    got = gpu_ops.select_pages(shifted, edges.cuda(), scale.cuda(), table.cuda(), lens.cuda(), 30, 16)
+    want = check(gpu_ops, q, edges, scale, table, lens, 30, 16)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_near_scores_are_told_apart(gpu_ops):
     """Pages whose scores differ only behind the 24 bits that a float32 sum keeps at its size, but not once rounded."""
     dim, pages = 128, 200
