@@ -70,3 +70,31 @@ def test_selected_bounds_are_upper_bounds_and_ties_go_low():
     flat = torch.zeros_like(q)  # every page scores 0
     table, _ = ref.select(flat, kv.k_bounds, kv.k_scale, kv.block_table, kv.seq_lens, 4, 16)
     assert table[0, 0].tolist() == kv.block_table[0, [0, 1, 2, 8]].tolist()
+
+
+def test_norm_is_the_library_norm_before_its_rounding():
+    g = torch.Generator().manual_seed(4)
+    x, r, w = (torch.randn(*s, generator=g, dtype=torch.float64) for s in ((5, 96), (5, 96), (96,)))
+    t, scale, res = ref.norm_fp8(x.float(), r.float(), w, eps=1e-5, group=32)
+    want = torch.nn.functional.rms_norm((x.float() + r.float()).double(), (96,), w, eps=1e-5)
+    torch.testing.assert_close((t.reshape(5, 3, 32) * scale[..., None]).reshape(5, 96), want)
+    torch.testing.assert_close(t.reshape(5, 3, 32).abs().amax(-1), torch.full((5, 3), 448.0, dtype=torch.float64))
+    assert torch.equal(res, x.float() + r.float())
+
+
+def test_append_to_empty_pages_is_the_quantised_cache():
+    g = torch.Generator().manual_seed(5)
+    lens = [16, 1, 40]
+    keys = [torch.randn(n, 2, 64, generator=g) for n in lens]
+    values = [3 * k.flip(0) for k in keys]
+    want = quantize_fp8_pages(build_paged_kv(keys, values, 16))
+    shape = want.k_cache.shape
+    cache = {n: torch.full(shape, float("nan"), dtype=torch.float64) for n in ("k", "v")}
+    cache |= {n + "_scale": torch.full(shape[::2], float("nan")) for n in ("k", "v")}
+    cache |= {"bounds": torch.zeros(shape[0], 2, 2, 64, dtype=torch.float64), "block_table": want.block_table}
+    ref.append(torch.cat(keys), torch.cat(values), cache, torch.tensor(lens), torch.tensor([0, 16, 17, 57]))
+    for name, codes, scales in (("k", want.k_cache, want.k_scale), ("v", want.v_cache, want.v_scale)):
+        torch.testing.assert_close(cache[name], codes.double(), rtol=0, atol=0, equal_nan=True)
+        torch.testing.assert_close(cache[name + "_scale"], scales, rtol=0, atol=0, equal_nan=True)
+    held = torch.cat([want.block_table[b, : (n + 15) // 16] for b, n in enumerate(lens)]).long()
+    torch.testing.assert_close(cache["bounds"][held], want.k_bounds.double()[held], rtol=0, atol=0)
