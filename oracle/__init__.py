@@ -32,10 +32,10 @@ Pinning (each check is in tests/test_oracle.py):
 
 * ``fp8_step`` (norms with FP8 output, the cache with page scales, append,
   selection, decode over both; in tests/test_oracle_fp8_step.py): its E4M3 rounding
-  against torch's conversion; the norm against F.rms_norm in float64; append at once
-  against append token by token and ``quantize_fp8_pages``; decode against
-  ``reference.paged_decode_attention_fp8`` with equal scales; bounds against the
-  keys that they bound.
+  against torch's conversion; the norm against a known answer and F.rms_norm in
+  float64; append against ``quantize_fp8_pages`` and, for repeated appends, the
+  unrounded values; decode against ``reference.paged_decode_attention_fp8`` with
+  equal scales; the selection's pinned pages and ties.
 
 There are no reference golden files to pin against: the original project's
 tests use seeded random data and the known answers above.
