@@ -225,8 +225,8 @@ constexpr bool kPageScaled = std::is_base_of_v<PageScaled, KVF>;
 
 // Cache policy of a segment's K/V loads. A head's row of 64 bytes is half a 128-byte
 // line whose other half is the next head's, so lines may stay for it: 32/8/64 B=64 of
-// 4,096 tokens 95 -> 90 us, up to 4,096 53 -> 46.5. (What bounds these is still the
-// number of 64-byte requests, as many as head_dim 128 makes of 128 bytes.)
+// 4,096 tokens 95 -> 90 us, up to 4,096 53 -> 46.5 (78.6 and 42.1 with the block loop's
+// end trimmed: block_loop).
 template <typename KVF, int D>
 constexpr int kLinePolicy() {
   return kPageScaled<KVF> && D * KVF::kBytes < 128 ? 0 : kKvPolicy;
@@ -428,6 +428,27 @@ constexpr int mfma_stages() {
   return D <= 64 ? (NT == 2 ? 4 : 6) : 2;
 }
 
+// The register pipeline's loop over a wave's blocks. With NS stages its body holds NS
+// blocks; a count that is no multiple leaves padding blocks at the end, which load nothing
+// but take a block's whole chain, about 1 us.
+//   kPadded   runs them;
+//   kTrimmed  leaves the body at the last block;
+//   kOneBody  (two stages) has one block in the body and copies the other's registers:
+//             half the instructions to fetch, which a short call notices.
+// Taken with scales per page only, each where it measured best (us, padded / trimmed / one
+// body). head_dim 64: 32/8 B=64 of 4,096 tokens 89.7 / 78.6, B=1 of 512 9.0 / 6.9. 128 and
+// one head tile: 32/8 B=64 of 4,096 92.0 / 91.2 / 89.1, 64/8 B=8 of 32,768 97.9 / 94.8 /
+// 93.6, B=4 of 1,024 10.7 / 9.7 / 9.8, 64 sequences' lists of 64 pages 30.4 / 29.3 / 28.9;
+// two: 32/1 up to 8,192 27.7 / 26.8 / 27.3. But balanced on four waves, more workgroups than
+// CUs: 8/1 B=300 of 2,048 40.0 / 41.7 / 43.8, 16/4 B=100 up to 2,048 32.1 / 32.7 / 33.8,
+// and at 256 32/8 B=32 of 4,096 89.9 / 90.8 / 93.2.
+enum class BlockLoop { kPadded, kTrimmed, kOneBody };
+template <typename KVF, int D, int NT>
+constexpr BlockLoop block_loop(bool balanced_four_waves = false) {
+  if (!kPageScaled<KVF> || D > 128 || (D == 128 && balanced_four_waves)) return BlockLoop::kPadded;
+  return D == 128 && NT == 1 ? BlockLoop::kOneBody : BlockLoop::kTrimmed;
+}
+
 // Waves of a one-unit uniform workgroup. fp32's MFMAs take several times the
 // cycles per cached byte that 16-bit ones do (a block of 16 tokens at head_dim
 // 128: 64 MFMAs of 32 cycles), and a workgroup has a CU to itself on most
@@ -435,18 +456,18 @@ constexpr int mfma_stages() {
 // waves per SIMD one computes while the other loads. Measured, 4 -> 8 waves:
 // 32/8/128 B=16 up to 4,096 tokens 75.6 -> 64.3 us, 64/8/128 B=16 up to 2,048
 // 44.8 -> 35.8, 32/8/128 B=64 of 512 tokens equal.
-template <typename E, int D, int NT>
+template <typename E, typename KVF, int D, int NT>
 constexpr int uniform_waves() {
-  return std::is_same_v<E, F32> && D <= 128 && NT == 1 ? 8 : kWaves;
+  return kEightWaves<KVF> || (std::is_same_v<E, F32> && D <= 128 && NT == 1) ? 8 : kWaves;
 }
 
 // Occupancy floor (waves per SIMD) handed to the register allocator. With two
 // head tiles (GQA groups of 17-32) the default allocation lands just above
 // the two-wave budget; asking for two keeps the accumulators in VGPRs, no
 // spills. Single-tile kernels run best at the allocator's own choice.
-template <int D, int NT, typename E = F16>
+template <int D, int NT, typename E = F16, typename KVF = E>
 constexpr int mfma_waves_per_eu() {
-  return (NT == 2 && !std::is_same_v<E, F32>) || uniform_waves<E, D, NT>() == 8 ? 2 : 1;
+  return (NT == 2 && !std::is_same_v<E, F32>) || uniform_waves<E, KVF, D, NT>() == 8 ? 2 : 1;
 }
 
 // Row of q (and of the output) that local head hl of unit u reads.
@@ -571,7 +592,8 @@ __device__ __forceinline__ void prefetch_window(const DecodeArgs& a, char* lds, 
 // qpre: the unit's Q fragments, already loaded by the caller (load_q), or
 // null. win_ready: the caller has issued this wave's first block-table window
 // loads for this segment (prefetch_window); LDS pipeline only.
-template <typename E, typename KVF, int D, int NT, int W = kWaves, int NSD = kDmaStages>
+template <typename E, typename KVF, int D, int NT, int W = kWaves, int NSD = kDmaStages,
+          BlockLoop LOOP = block_loop<KVF, D, NT>()>
 __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, const Unit& u, const Dest& dst,
                                              const int wave, const QFrag<NT, qk_chunks<E, D>()>* qpre = nullptr,
                                              const bool win_ready = false) {
@@ -1223,10 +1245,29 @@ __device__ __forceinline__ void mfma_segment(const DecodeArgs& a, char* lds, con
     };
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) load_slot(first_src(min(s, nblk - 1)), s, s < nblk);
-    for (int base = 0; base < nblk; base += NS) {
+    if constexpr (LOOP == BlockLoop::kOneBody) {
+      static_assert(NS == 2 && PS, "one body copies one stage");
+      auto ahead = pg[1], behind = pg[0];  // the entries of blocks i + 1 and i + 2
+#pragma unroll 1
+      for (int i = 0; i < nblk; ++i) {
+        const auto next = block_src(min(i + 1, nblk - 1), ahead);
+        ahead = behind;
+        behind = table_load(min(i + 3, nblk - 1));
+        load_slot(next, 1, i + 1 < nblk);
+        process_block(i, kb[0], vb[0], std::false_type{}, sb[0]);
+#pragma unroll
+        for (int c = 0; c < NL; ++c) {
+          kb[0][c] = kb[1][c];
+          vb[0][c] = vb[1][c];
+        }
+        sb[0] = sb[1];
+      }
+    }
+    for (int base = 0; base < (LOOP == BlockLoop::kOneBody ? 0 : nblk); base += NS) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const int i = base + s;
+        if (LOOP == BlockLoop::kTrimmed && s > 0 && i >= nblk) break;
         const int slot = (s + NS - 1) % NS;  // block i + NS - 1 (base is a multiple of NS)
         const int j = min(i + NS - 1, nblk - 1);
         const auto next = block_src(j, pg[slot]);
@@ -1540,9 +1581,9 @@ __device__ __forceinline__ Dest uniform_dest(const DecodeArgs& a, const Unit& u,
 // Uniform splits: workgroup = (sequence, KV head, head group, split), the
 // split owning pages_per_split pages (the reference's decomposition).
 template <typename E, typename KVF, int D, int NT>
-__global__ void __launch_bounds__((uniform_waves<E, D, NT>() * 64), (mfma_waves_per_eu<D, NT, E>()))
+__global__ void __launch_bounds__((uniform_waves<E, KVF, D, NT>() * 64), (mfma_waves_per_eu<D, NT, E, KVF>()))
     decode_mfma_kernel(const DecodeArgs a) {
-  constexpr int W = uniform_waves<E, D, NT>();
+  constexpr int W = uniform_waves<E, KVF, D, NT>();
   __shared__ __attribute__((
       aligned(16))) char lds[MfmaLds<D, NT, W, dma_staged<KVF, D, NT>(), kDmaStages, E::kBytes>::kBytes];
   __shared__ int s_last[1];
@@ -1939,6 +1980,7 @@ __global__ void __launch_bounds__((PAIR * balanced_waves<KVF>() * 64),
                                   (balanced_waves_per_eu<KVF, D, NT, PAIR>()))
     decode_mfma_balanced_kernel(const DecodeArgs a) {
   constexpr int W = balanced_waves<KVF>();
+  constexpr BlockLoop kLoop = block_loop<KVF, D, NT>(PAIR * W == kWaves);
   using Lds = MfmaLds<D, NT, W, dma_staged<KVF, D, NT>()>;
   __shared__ __attribute__((aligned(16))) char lds[PAIR * Lds::kBytes];
   __shared__ int s_last[PAIR];
@@ -1978,7 +2020,7 @@ __global__ void __launch_bounds__((PAIR * balanced_waves<KVF>() * 64),
       gu.page_end = n;
       Dest dst{};
       dst.final = true;
-      mfma_segment<E, KVF, D, NT, W>(a, lds + half * Lds::kBytes, gu, dst, hw, &gq, true);
+      mfma_segment<E, KVF, D, NT, W, kDmaStages, kLoop>(a, lds + half * Lds::kBytes, gu, dst, hw, &gq, true);
       return;
     }
     wait_vmcnt<0>();  // the guessed window loads write LDS the segments below reuse
@@ -2052,7 +2094,7 @@ __global__ void __launch_bounds__((PAIR * balanced_waves<KVF>() * 64),
       // The previous segment's waves may still read LDS; before the first
       // segment nothing has used it (the schedule needs no LDS), so no barrier.
       if (pos != st.pos) __syncthreads();
-      mfma_segment<E, KVF, D, NT, W>(a, lds + half * Lds::kBytes, u, dst, hw);
+      mfma_segment<E, KVF, D, NT, W, kDmaStages, kLoop>(a, lds + half * Lds::kBytes, u, dst, hw);
       if (NT == 1 && !dst.final && a.arrivals != nullptr) {  // see kFusedMergeMaxHeads
         // The unit's segments are workgroups w0 .. w1, those whose ranges hold
         // its first and last page (slots (w + list unit) * PAIR + half).
@@ -3237,6 +3279,10 @@ int launch_valu(const DecodeArgs& a, int head_dim, unsigned grid, hipStream_t st
   return fail(KL_ERR_UNSUPPORTED, "no kernel for this head_dim");
 }
 
+// Whether an unpaired launch of an FP8 cache at head_dim 128 takes eight waves per unit
+// (balanced_waves; uniform splits: with scales per page).
+bool wide_fp8(unsigned grid) { return static_cast<int64_t>(grid) <= current_cu_count(); }
+
 // grid: the number of units (sequences x KV heads x head groups x splits);
 // paired launches take two units per workgroup, so grid must then be even.
 template <typename E, typename KVF>
@@ -3257,7 +3303,17 @@ int launch_uniform_mfma(const DecodeArgs& a, int head_dim, unsigned grid, hipStr
           return fail(KL_ERR_UNSUPPORTED, "paired decode needs 16-bit queries, whole blocks per page and head_dim <= 128");
         }
       } else {
-        decode_mfma_kernel<E, KVF, D, NT><<<grid, uniform_waves<E, D, NT>() * 64, 0, stream>>>(a);
+        // A workgroup that has a CU to itself takes eight waves, as in launch_balanced.
+        // Measured (us, 4 -> 8): 32 sequences' lists of 128 pages, 32/8 31.3 -> 25.4, of
+        // 16 pages 7.8 -> 7.2, 32/8 B=1 of 16,384 tokens 15.5 -> 13.7.
+        if constexpr (kPageScaled<KVF> && D == 128) {
+          if (wide_fp8(grid)) {
+            using W8 = EightWaves<KVF>;
+            decode_mfma_kernel<E, W8, D, NT><<<grid, uniform_waves<E, W8, D, NT>() * 64, 0, stream>>>(a);
+            return KL_OK;
+          }
+        }
+        decode_mfma_kernel<E, KVF, D, NT><<<grid, uniform_waves<E, KVF, D, NT>() * 64, 0, stream>>>(a);
       }
       return KL_OK;
     } else {
@@ -3278,10 +3334,6 @@ int balanced_charge(int page_size, int head_dim, int kv_bytes, int paired, int h
   return static_cast<int>(
       std::min<int64_t>(kMaxSegmentCharge, cdiv(kSegmentStartBytes + 2 * partial_bytes, page_bytes)));
 }
-
-// Whether an unpaired balanced launch of an FP8 cache at head_dim 128 takes eight
-// waves per unit (balanced_waves).
-bool wide_fp8(const DecodeArgs& a) { return a.grid <= current_cu_count(); }
 
 template <typename E, typename KVF>
 int launch_balanced(DecodeArgs a, int head_dim, hipStream_t stream) {
@@ -3307,7 +3359,7 @@ int launch_balanced(DecodeArgs a, int head_dim, hipStream_t stream) {
         }
       } else {
         if constexpr (KVF::kBytes == 1 && D == 128) {
-          if (wide_fp8(a)) {
+          if (wide_fp8(grid)) {
             using W8 = EightWaves<KVF>;
             decode_mfma_balanced_kernel<E, W8, D, NT, 1><<<grid, balanced_waves<W8>() * 64, 0, stream>>>(a);
             return KL_OK;
