@@ -509,26 +509,60 @@ struct ScoreQueries {
       }
     }
   }
+  // max_g sum_d |q_gd|, in every lane.
+  __device__ __forceinline__ float size() const {
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C / 2; ++c) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const auto w = __builtin_bit_cast(Pack<typename E::S, 2>, v[c][half][i] | v[c + C / 2][half][i]);
+          sum += fabsf(E::to_f32(w.v[0])) + fabsf(E::to_f32(w.v[1]));
+        }
+      }
+    }
+    return row16_max(sum_xor32(sum_xor16(sum)));
+  }
+};
+
+// What steps 2 and 3 need to know of a unit beside its keys, each lane's share of it.
+struct Seen {
+  float scale = 0.0f;                     // largest k_scale
+  float size = 0.0f;                      // max_g sum_d |q_gd|
+  uint32_t low = 0xffffffffu, high = 0;  // smallest and largest key
+  __device__ __forceinline__ void add(uint32_t key) {
+    low = min(low, key);
+    high = max(high, key);
+  }
 };
 
 // Step 1 for a unit's tiles first, first + step, ..., by a wave: store(page, key) by lanes
-// 0 .. 15, and scale(tile, largest k_scale of its pages) in every lane.
+// 0 .. 15, and tile_scale(tile, largest k_scale of its pages) in every lane. The result is
+// the queries' size, of waves that have a tile.
 //
 // What bounds it: the bounds of a unit arrive at a CU's share of HBM bandwidth, 256 KiB
 // for 1,024 pages of head_dim 128 (11 us on one CU), so a unit's tiles are spread over
-// several workgroups. Loading a tile ahead gained nothing.
+// several workgroups; a tile is two dependent loads, its pages' ids and their bounds, so
+// the next tile's ids are loaded ahead (us: 8 x 8 units of 1,024 pages 15.7 -> 15.0; its
+// bounds, too: 14.9, and others slower).
 template <typename E, int D, typename Store, typename Scale>
-__device__ __forceinline__ void score_unit(const SelectArgs& a, int64_t unit, int b, int h, int pages, int first,
-                                           int step, Store&& store, Scale&& tile_scale) {
+__device__ __forceinline__ float score_unit(const SelectArgs& a, int64_t unit, int b, int h, int pages, int first,
+                                            int step, Store&& store, Scale&& tile_scale) {
   constexpr int C = 2 * D / 64;  // loads of 16 bytes a lane for a tile
   const int lane = __lane_id(), k = lane >> 4;
   const int tiles = (pages + kTile - 1) / kTile;
-  if (first >= tiles) return;
+  if (first >= tiles) return 0.0f;
   const int32_t* table = a.table + b * a.bt_stride;
+  auto id_of = [&](int tile) { return table[min(kTile * tile + (lane & 15), pages - 1)]; };
+  int id = id_of(first);
+  float size = 0.0f;
   ScoreQueries<E, D> q(a, unit, 0);
   for (int tile = first; tile < tiles; tile += step) {
     const int page = kTile * tile + (lane & 15);
-    const int64_t head = static_cast<int64_t>(table[min(page, pages - 1)]) * a.heads + h;
+    const int64_t head = static_cast<int64_t>(id) * a.heads + h;
+    id = id_of(tile + step);
     const uint8_t* edge = a.bounds + head * (2 * D) + 16 * k;
     u32x4 w[C];
 #pragma unroll
@@ -538,6 +572,7 @@ __device__ __forceinline__ void score_unit(const SelectArgs& a, int64_t unit, in
     bool finite = true;
     for (int g0 = 0; g0 < a.group; g0 += kHeadsAtOnce) {
       if (a.group > kHeadsAtOnce) q = ScoreQueries<E, D>(a, unit, g0);
+      if (tile == first) size = fmaxf(size, q.size());
       f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < C; ++c) {
@@ -562,6 +597,7 @@ __device__ __forceinline__ void score_unit(const SelectArgs& a, int64_t unit, in
     if (k == 0 && page < pages) store(page, key);
     tile_scale(tile, row16_max(scale));
   }
+  return size;
 }
 
 // How far step 1's score may be from the true one, over the sum of its terms' sizes: a
@@ -582,35 +618,56 @@ __device__ __forceinline__ float query_size(const SelectArgs& a, int64_t unit, i
   return most;
 }
 
-// The true score's key of a page, by a wave: each row of 16 lanes a query head, each
-// lane D / 16 dimensions.
-template <typename E, int D>
-__device__ __forceinline__ uint32_t true_key(const SelectArgs& a, int64_t unit, int b, int h, int page) {
+// The true score's key of a page, `head` its index in k_scale: ROWS by a row of 16 lanes
+// (each row a page of its own), else by a wave (each row another query head). Each lane
+// has D / 16 dimensions.
+template <typename E, int D, bool ROWS>
+__device__ __forceinline__ uint32_t true_key(const SelectArgs& a, int64_t unit, int64_t head) {
   constexpr int N = D / 16;
   const int lane = __lane_id(), d0 = N * (lane & 15);
-  const int64_t head = static_cast<int64_t>(a.table[b * a.bt_stride + page]) * a.heads + h;
-  const uint8_t* edge = a.bounds + head * (2 * D) + d0;
+  const auto* edge = reinterpret_cast<const uint32_t*>(a.bounds + head * (2 * D) + d0);
+  uint32_t words[2][N / 4];
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    words[0][i] = edge[i];
+    words[1][i] = edge[D / 4 + i];
+  }
   const double scale = a.scale[head];
   double best = -INFINITY;
   for (int g0 = 0; g0 < a.group; g0 += 4) {
-    const int g = g0 + (lane >> 4);
-    const auto* q = static_cast<const typename E::S*>(a.q) + (unit * a.group + min(g, a.group - 1)) * D + d0;
-    double sum = 0.0;
+    // Four heads one after the other, their loads together, or one in each row.
+    constexpr int kHeads = ROWS ? 4 : 1;
+    Pack<typename E::S, N> qs[kHeads];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float v = E::to_f32(q[i]);
-      sum = fma(static_cast<double>(v < 0.0f ? v : 0.0f), static_cast<double>(e4m3_value(edge[i])), sum);
-      sum = fma(static_cast<double>(v < 0.0f ? 0.0f : v), static_cast<double>(e4m3_value(edge[D + i])), sum);
+    for (int n = 0; n < kHeads; ++n) {
+      const int g = min(g0 + (ROWS ? n : lane >> 4), a.group - 1);
+      __builtin_memcpy(&qs[n], static_cast<const typename E::S*>(a.q) + (unit * a.group + g) * D + d0, sizeof(qs[n]));
     }
-    sum += dpp64<kDppQuadSwap1>(sum);
-    sum += dpp64<kDppQuadSwap2>(sum);
-    sum += dpp64<kDppRowRor4>(sum);
-    sum += dpp64<kDppRowRor8>(sum);
-    if (g < a.group) best = max_or_nan(sum, best);
+#pragma unroll
+    for (int n = 0; n < kHeads; ++n) {
+      double sum = 0.0;
+      static_for<N>([&](auto i) {
+        constexpr int I = decltype(i)::value;
+        const float v = E::to_f32(qs[n].v[I]);
+        sum = fma(static_cast<double>(v < 0.0f ? v : 0.0f), static_cast<double>(e4m3_value_at<I % 4>(words[0][I / 4])), sum);
+        sum = fma(static_cast<double>(v < 0.0f ? 0.0f : v), static_cast<double>(e4m3_value_at<I % 4>(words[1][I / 4])), sum);
+      });
+      sum += dpp64<kDppQuadSwap1>(sum);
+      sum += dpp64<kDppQuadSwap2>(sum);
+      sum += dpp64<kDppRowRor4>(sum);
+      sum += dpp64<kDppRowRor8>(sum);
+      best = max_or_nan(sum, best);  // (the last head of a group again changes nothing)
+    }
   }
-  for (int m = 16; m <= 32; m *= 2) best = max_or_nan(best, __shfl_xor(best, m));
+  if constexpr (!ROWS) {
+    for (int m = 16; m <= 32; m *= 2) best = max_or_nan(best, __shfl_xor(best, m));
+  }
   return score_key(static_cast<float>(best * scale));
 }
+
+// Query heads up to which a page between has a row of lanes: four pages a wave then share
+// a round trip to memory.
+constexpr int kRowsGroup = 8;
 
 // Workgroups of W waves (W = 8 or 16: see wide_workgroups).
 constexpr int kListed = 64;  // pages between that a wave ranks
@@ -620,11 +677,11 @@ struct PickLds {
   static constexpr int kBins = 64 * W;
   int count[2][3][W];  // of two rounds in turn, so that a round needs one barrier
   float scale[W], size[W];
-  uint32_t low[W], high[W];
-  int bins[kBins];
-  int bin;                    // that holds T
+  uint32_t not_low[W], high[W];
+  alignas(16) int bins[kBins];
   int kept, between;          // pages certainly kept, pages between
-  int list[kListed];          // the first of them, and their keys
+  int list[kListed];          // the first of them, their ids and their keys
+  int list_id[kListed];
   uint32_t list_key[kListed];
 };
 
@@ -678,11 +735,27 @@ __device__ uint32_t smallest_kept(PickLds<W>& lds, int want, int q0, int free1, 
   return low;
 }
 
-// Steps 2 and 3, by a workgroup: a unit's pages from its keys. scale: the
-// largest k_scale that the lane has seen of the unit's pages.
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+  v = max(v, dpp_u32<kDppQuadSwap1>(v));
+  v = max(v, dpp_u32<kDppQuadSwap2>(v));
+  v = max(v, dpp_u32<kDppRowRor4>(v));
+  return max(v, dpp_u32<kDppRowRor8>(v));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = row16_max(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+  const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(static_cast<uint32_t>(s[0]), static_cast<uint32_t>(s[1]));
+}
+
+// Steps 2 and 3, by a workgroup: a unit's pages from its keys.
+//
+// What bounds it: its barriers and LDS round trips, five of them where nothing is tied,
+// and one round trip to memory for the pages between. About 5 us of 1,024 pages.
 template <typename E, int D, int W>
 __device__ void pick_pages(const SelectArgs& a, PickLds<W>& lds, int64_t unit, int b, int h, int pages, uint32_t* keys,
-                           float scale) {
+                           const Seen& seen) {
   constexpr int kBins = PickLds<W>::kBins;
   const int wave = wave_id(), lane = __lane_id();
   const int kept = a.keep;  // < pages
@@ -692,36 +765,24 @@ __device__ void pick_pages(const SelectArgs& a, PickLds<W>& lds, int64_t unit, i
   const int q0 = free0 + static_cast<int>(threadIdx.x);
   const int want = kept - a.first - a.last;
   auto key = [&](int p) { return keys[p]; };
+  // Where the last step's pages begin, and the ids of this thread's first pages, there
+  // and in step 3, on their way.
+  const int range = (pages + 64 * W - 1) / (64 * W) * 64;
+  const int p0 = min(wave * range, pages), p1 = min(p0 + range, pages);
+  const int id_p0 = table[min(p0 + lane, pages - 1)];
+  const int id_q0 = table[min(q0, pages - 1)];
 
-  scale = max_xor32(max_xor16(row16_max(scale)));
-  const float size = query_size<E, D>(a, unit, wave, W);
+  const float wave_scale = max_xor32(max_xor16(row16_max(seen.scale)));
+  const uint32_t wave_not_low = wave_max(~seen.low), wave_high = wave_max(seen.high);
   if (lane == 0) {
-    lds.scale[wave] = scale;
-    lds.size[wave] = size;
+    lds.scale[wave] = wave_scale;
+    lds.size[wave] = seen.size;
+    lds.not_low[wave] = wave_not_low;
+    lds.high[wave] = wave_high;
   }
   __syncthreads();  // the keys are there, too
-  uint32_t low = 0xffffffffu, high = 0;
-  for (int p = q0; p < free1; p += 64 * W) {
-    low = min(low, key(p));
-    high = max(high, key(p));
-  }
-  for (int m = 32; m > 0; m >>= 1) {
-    low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), m)));
-    high = max(high, static_cast<uint32_t>(__shfl_xor(static_cast<int>(high), m)));
-  }
-  if (lane == 0) {
-    lds.low[wave] = low;
-    lds.high[wave] = high;
-  }
-  __syncthreads();
-  low = lds.low[lane % W];
-  high = lds.high[lane % W];
-  scale = row16_max(lds.scale[lane % W]);
-  const float most_size = row16_max(lds.size[lane % W]);
-  for (int m = W / 2; m > 0; m >>= 1) {
-    low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), m)));
-    high = max(high, static_cast<uint32_t>(__shfl_xor(static_cast<int>(high), m)));
-  }
+  const float scale = row16_max(lds.scale[lane % W]), most_size = row16_max(lds.size[lane % W]);
+  const uint32_t low = ~row16_max(lds.not_low[lane % W]), high = row16_max(lds.high[lane % W]);
   uint32_t least = 0xffffffffu;  // the smallest key kept: none but the pinned pages
   if (want > 0) {
     // Step 2. What underflows in 16 bits adds less than the last term.
@@ -735,51 +796,79 @@ __device__ void pick_pages(const SelectArgs& a, PickLds<W>& lds, int64_t unit, i
     if (finite) {
       for (int p = q0; p < free1; p += 64 * W) atomicAdd(&lds.bins[min(bin_of(key_score(key(p))), kBins - 1)], 1);
       __syncthreads();
-      // Thread t has bin kBins - 1 - t; the pages from it upwards.
-      const int mine = lds.bins[kBins - 1 - static_cast<int>(threadIdx.x)];
-      int upto = wave_prefix_sum(mine);
-      if (lane == 63) lds.count[0][0][wave] = upto;
-      __syncthreads();
-      const int ahead = lane < wave ? lds.count[0][0][lane % W] : 0;
-      upto += __builtin_amdgcn_readlane(wave_prefix_sum(ahead), 63);
-      if (upto >= want && upto - mine < want) lds.bin = kBins - 1 - static_cast<int>(threadIdx.x);
-      __syncthreads();
-      bin = lds.bin;
+      // Lane l has the W bins below kBins - W l; every wave finds the bin by itself.
+      int n[W], mine = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        n[i] = lds.bins[kBins - W * (lane + 1) + i];
+        mine += n[i];
+      }
+      const int upto = wave_prefix_sum(mine);
+      int left = want - (upto - mine), at = 0;
+#pragma unroll
+      for (int i = W - 1; i >= 0; --i) {
+        if (left > 0) at = i;
+        left -= n[i];
+      }
+      const uint64_t here = __ballot(upto >= want && upto - mine < want);
+      const int owner = __builtin_ctzll(here);
+      bin = kBins - W * (owner + 1) + __builtin_amdgcn_readlane(at, owner);
     }
     // Step 3. The pages between are listed in the order that they come in; which of them
     // are kept does not depend on it. (The last bin takes what is past its end, too.)
-    for (int p = q0; p < free1; p += 64 * W) {
-      const float s = key_score(key(p));
-      if (finite && bin < kBins - 1 && bin_of(s - reach) > bin) {
-        keys[p] = kKeyKept;
-        atomicAdd(&lds.kept, 1);
-      } else if (finite && bin_of(s + reach) < bin) {
-        keys[p] = 0;
-      } else {
-        keys[p] = kKeyNotFinite;  // to be scored
-        const int i = atomicAdd(&lds.between, 1);
-        if (i < kListed) lds.list[i] = p;
+    int sure = 0;
+    for (int base = 0; base < free1 - free0; base += 64 * W) {
+      const int p = q0 + base;
+      const bool valid = p < free1;
+      const float s = valid ? key_score(key(p)) : 0.0f;
+      const bool above = valid && finite && bin < kBins - 1 && bin_of(s - reach) > bin;
+      const bool below = finite && bin_of(s + reach) < bin;
+      sure += __builtin_popcountll(__ballot(above));
+      if (valid) {
+        keys[p] = above ? kKeyKept : below ? 0 : kKeyNotFinite;  // the last: to be scored
+        if (!above && !below) {
+          const int i = atomicAdd(&lds.between, 1);
+          if (i < kListed) {
+            lds.list[i] = p;
+            lds.list_id[i] = base == 0 ? id_q0 : table[p];
+          }
+        }
       }
     }
+    if (lane == 0 && sure > 0) atomicAdd(&lds.kept, sure);
     __syncthreads();
     const int between = lds.between;
     if (between <= kListed) {
-      for (int i = wave; i < between; i += W) {
-        const uint32_t k = true_key<E, D>(a, unit, b, h, __builtin_amdgcn_readfirstlane(lds.list[i]));
-        if (lane == 0) lds.list_key[i] = k;
+      if (a.group <= kRowsGroup) {
+        for (int i0 = 4 * wave; i0 < between; i0 += 4 * W) {
+          const int i = i0 + (lane >> 4);
+          const uint32_t k = true_key<E, D, true>(
+              a, unit, static_cast<int64_t>(lds.list_id[min(i, between - 1)]) * a.heads + h);
+          if ((lane & 15) == 0 && i < between) lds.list_key[i] = k;
+        }
+      } else {
+        for (int i = wave; i < between; i += W) {
+          const int id = __builtin_amdgcn_readfirstlane(lds.list_id[i]);
+          const uint32_t k = true_key<E, D, false>(a, unit, static_cast<int64_t>(id) * a.heads + h);
+          if (lane == 0) lds.list_key[i] = k;
+        }
       }
       __syncthreads();
-      if (wave == 0) {
-        const bool mine = lane < between;
-        const int p = mine ? lds.list[lane] : 0;
-        const uint32_t k = mine ? lds.list_key[lane] : 0;
+      // A row of lanes ranks a page: the ones before it are counted 16 at a time.
+      for (int i0 = 4 * wave; i0 < between; i0 += 4 * W) {
+        const int i = min(i0 + (lane >> 4), between - 1);
+        const int p = lds.list[i];
+        const uint32_t k = lds.list_key[i];
         int better = 0;
-        for (int i = 0; i < between; ++i) {
-          const uint32_t ki = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k), i));
-          const int pi = __builtin_amdgcn_readlane(p, i);
-          better += ki > k || (ki == k && pi < p) ? 1 : 0;
+        for (int j = lane & 15; j < between; j += 16) {
+          const uint32_t kj = lds.list_key[j];
+          better += kj > k || (kj == k && lds.list[j] < p) ? 1 : 0;
         }
-        if (mine) keys[p] = better < want - lds.kept ? kKeyKept : 0;
+        better += static_cast<int>(dpp_u32<kDppQuadSwap1>(better));
+        better += static_cast<int>(dpp_u32<kDppQuadSwap2>(better));
+        better += static_cast<int>(dpp_u32<kDppRowRor4>(better));
+        better += static_cast<int>(dpp_u32<kDppRowRor8>(better));
+        if ((lane & 15) == 0) keys[p] = better < want - lds.kept ? kKeyKept : 0;
       }
       __syncthreads();
       least = kKeyKept;
@@ -789,7 +878,7 @@ __device__ void pick_pages(const SelectArgs& a, PickLds<W>& lds, int64_t unit, i
         uint64_t todo = __ballot(p >= free0 && p < free1 && keys[min(p, pages - 1)] == kKeyNotFinite);
         for (; todo != 0; todo &= todo - 1) {
           const int at = base + __builtin_ctzll(todo);
-          const uint32_t k = true_key<E, D>(a, unit, b, h, at);
+          const uint32_t k = true_key<E, D, false>(a, unit, static_cast<int64_t>(table[at]) * a.heads + h);
           if (lane == 0) keys[at] = k;
         }
       }
@@ -800,8 +889,6 @@ __device__ void pick_pages(const SelectArgs& a, PickLds<W>& lds, int64_t unit, i
 
   // Positions: pages above the smallest key kept, and the first ones equal to it. A wave
   // has neighbouring pages, 64 at a time, whose ranks are counts of lanes below.
-  const int range = (pages + 64 * W - 1) / (64 * W) * 64;
-  const int p0 = min(wave * range, pages), p1 = min(p0 + range, pages);
   auto ranked = [&](auto&& take) {
     for (int base = p0; base < p1; base += 64) {
       const int p = base + lane;
@@ -833,7 +920,9 @@ __device__ void pick_pages(const SelectArgs& a, PickLds<W>& lds, int64_t unit, i
   ranked([&](int p, uint64_t over, uint64_t tie) {
     const int ties_here = ties_at + __builtin_popcountll(tie & below);
     const int at = above_at + __builtin_popcountll(over & below) + min(ties_here, room);
-    if ((over & mine) != 0 || ((tie & mine) != 0 && ties_here < room)) out[at] = table[p];
+    if ((over & mine) != 0 || ((tie & mine) != 0 && ties_here < room)) {
+      out[at] = p < p0 + 64 ? id_p0 : table[p];
+    }
     above_at += __builtin_popcountll(over);
     ties_at += __builtin_popcountll(tie);
   });
@@ -878,14 +967,19 @@ __global__ void __launch_bounds__(64 * W) select_kernel(const SelectArgs a) {
   if (static_cast<int>(blockIdx.x) >= wgs) return;
   clear(lds);
   const int first = static_cast<int>(blockIdx.x) * W + wave_id(), step = wgs * W;
-  float scale = 0.0f;
+  Seen seen;
   if (wgs == 1) {
-    score_unit<E, D>(a, unit, b, h, pages, first, step, [&](int page, uint32_t key) { keys[page] = key; },
-                     [&](int, float s) { scale = fmaxf(scale, s); });
+    seen.size = score_unit<E, D>(
+        a, unit, b, h, pages, first, step,
+        [&](int page, uint32_t key) {
+          keys[page] = key;
+          seen.add(key);
+        },
+        [&](int, float s) { seen.scale = fmaxf(seen.scale, s); });
   } else {
     uint32_t* shared = a.keys + unit * unit_words(a.max_pages);
     const auto rsrc = make_rsrc(uniform_ptr(shared));
-    score_unit<E, D>(
+    seen.size = score_unit<E, D>(
         a, unit, b, h, pages, first, step,
         [&](int page, uint32_t key) {
           buffer_store_f32<kCachePolicyDevice>(rsrc, static_cast<uint32_t>(page) * 4u, __builtin_bit_cast(float, key));
@@ -906,14 +1000,16 @@ __global__ void __launch_bounds__(64 * W) select_kernel(const SelectArgs a) {
     if (!__builtin_amdgcn_readfirstlane(s_last)) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");  // no load moves above the arrival
     for (int p = threadIdx.x; p < pages; p += 64 * W) {
-      keys[p] = __builtin_bit_cast(uint32_t, buffer_load_f32<kCachePolicyDevice>(rsrc, static_cast<uint32_t>(p) * 4u));
+      const uint32_t k = __builtin_bit_cast(uint32_t, buffer_load_f32<kCachePolicyDevice>(rsrc, static_cast<uint32_t>(p) * 4u));
+      keys[p] = k;
+      seen.add(k);
     }
     for (int t = threadIdx.x; t < tiles; t += 64 * W) {
-      scale = fmaxf(scale, buffer_load_f32<kCachePolicyDevice>(rsrc, static_cast<uint32_t>(a.max_pages + t) * 4u));
+      seen.scale = fmaxf(seen.scale, buffer_load_f32<kCachePolicyDevice>(rsrc, static_cast<uint32_t>(a.max_pages + t) * 4u));
     }
   }
   write_len(a, unit, len, pages);
-  pick_pages<E, D, W>(a, lds, unit, b, h, pages, keys, scale);
+  pick_pages<E, D, W>(a, lds, unit, b, h, pages, keys, seen);
 }
 
 // The same in two launches: for tables past kLdsPages, and where there are no counters.
@@ -948,15 +1044,20 @@ __global__ void __launch_bounds__(64 * W) pick_kernel(const SelectArgs a) {
   }
   clear(lds);
   uint32_t* shared = a.keys + unit * unit_words(a.max_pages);
-  float scale = 0.0f;
+  Seen seen;
+  seen.size = query_size<E, D>(a, unit, wave_id(), W);
   for (int t = threadIdx.x; t < (pages + kTile - 1) / kTile; t += 64 * W) {
-    scale = fmaxf(scale, __builtin_bit_cast(float, shared[a.max_pages + t]));
+    seen.scale = fmaxf(seen.scale, __builtin_bit_cast(float, shared[a.max_pages + t]));
+  }
+  for (int p = threadIdx.x; p < pages; p += 64 * W) {
+    const uint32_t k = shared[p];
+    if (pages <= kLdsPages) keys[p] = k;
+    seen.add(k);
   }
   if (pages <= kLdsPages) {
-    for (int p = threadIdx.x; p < pages; p += 64 * W) keys[p] = shared[p];
-    pick_pages<E, D, W>(a, lds, unit, b, h, pages, keys, scale);
+    pick_pages<E, D, W>(a, lds, unit, b, h, pages, keys, seen);
   } else {
-    pick_pages<E, D, W>(a, lds, unit, b, h, pages, shared, scale);
+    pick_pages<E, D, W>(a, lds, unit, b, h, pages, shared, seen);
   }
 }
 
