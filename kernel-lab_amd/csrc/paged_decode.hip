@@ -3471,8 +3471,8 @@ int decode_entry(kl_dtype dtype, Cache cache, void* out, const void* q, const vo
   const bool use_mfma = kv8 || !opt.force_valu();
   // Tables per KV head hold about as many pages each (kl_select_pages gives every one
   // the same number at most), so a full batch takes one uniform split. Measured (us,
-  // balanced -> uniform, 32 query heads over 8): 32 sequences of 128 pages of 16 35.0 ->
-  // 28.2, 64 of 64 pages 35.2 -> 30.4.
+  // balanced -> uniform on four waves, 32 query heads over 8): 32 sequences of 128 pages
+  // of 16 35.0 -> 28.2, 64 of 64 pages 35.2 -> 30.4.
   if (cache == Cache::kPageScalesHeadTables && num_splits == 0 && opt.balance() < 0 &&
       static_cast<int64_t>(batch) * cdiv(num_q_heads, mfma_heads_cap(num_q_heads, head_dim)) >= current_cu_count()) {
     num_splits = 1;
