@@ -75,6 +75,48 @@ def test_splits_and_balanced_schedule(gpu_ops, num_splits, dtype, hq, hkv):
     dense(gpu_ops, *problem([5000, 3, 700, 64], hq, hkv, 128, dtype, seed=2), num_splits=num_splits)
 
 
+@pytest.mark.parametrize("num_splits", [0, 1, 2, -1])
+@pytest.mark.parametrize(("hq", "hkv", "head_dim"), [(8, 2, 64), (32, 1, 64), (8, 2, 128), (32, 1, 128), (20, 5, 128), (4, 1, 256)])
+def test_every_number_of_blocks(gpu_ops, hq, hkv, head_dim, num_splits):
+    """Waves with every number of blocks up to some pipelines' length, alone and beside other sequences."""
+    lens = [16 * n - n % 5 for n in range(1, 51)]
+    q, kv = problem(lens, hq, hkv, head_dim, torch.bfloat16, seed=head_dim)
+    dense(gpu_ops, q, kv, num_splits=num_splits)
+    c = on_gpu(kv)
+    want, size = ref.decode(q, kv.k_cache, kv.v_cache, kv.block_table, kv.seq_lens, kv.k_scale, kv.v_scale)
+    for b in (0, 1, 2, 6, 7, 8, 15, 16, 24, 31, 32, 49):
+        got = gpu_ops.paged_decode_attention(q[b : b + 1].cuda(), c.k_cache, c.v_cache, c.block_table[b : b + 1], c.seq_lens[b : b + 1],
+                                             k_scale=c.k_scale, v_scale=c.v_scale, num_splits=num_splits)
+        check(got, want[b : b + 1], size[b : b + 1], q.dtype)
+
+
+def test_pages_far_into_a_large_cache(gpu_ops):
+    """Page offsets past 2^32 bytes, through a table of the sequence and through tables per head that were selected."""
+    heads, dim, page, last = 8, 256, 128, 5
+    pages = (1 << 32) // (heads * dim * page) + 10
+    q, kv = problem([page * last - 3], 16, heads, dim, torch.bfloat16, page=page, seed=6)
+    where = torch.arange(pages - last, pages)
+    wide = {n: torch.zeros(pages, *getattr(kv, n).shape[1:], dtype=getattr(kv, n).dtype, device="cuda")
+            for n in ("k_cache", "v_cache", "k_scale", "v_scale", "k_bounds")}
+    held = kv.block_table[0, :last].long()
+    for name, t in wide.items():
+        bits = getattr(kv, name)[held]
+        (t.view(torch.uint8) if t.element_size() == 1 else t)[where.cuda()] = (bits.view(torch.uint8) if t.element_size() == 1 else bits).cuda()
+    table = where.to(torch.int32)[None].cuda()
+    lens = kv.seq_lens.cuda()
+    want = ref.decode(q, kv.k_cache, kv.v_cache, kv.block_table, kv.seq_lens, kv.k_scale, kv.v_scale)
+    got = gpu_ops.paged_decode_attention(q.cuda(), wide["k_cache"], wide["v_cache"], table, lens, k_scale=wide["k_scale"], v_scale=wide["v_scale"])
+    check(got, *want, q.dtype)
+    some = gpu_ops.select_pages(q.cuda(), wide["k_bounds"], wide["k_scale"], table, lens, 3, page)
+    chosen = ref.select(q, kv.k_bounds, kv.k_scale, kv.block_table, kv.seq_lens, 3, page)
+    place = {int(p): i for i, p in enumerate(held.tolist())}
+    assert torch.equal(some[0].cpu() - (pages - last), chosen[0].apply_(lambda p: place[int(p)]))
+    assert torch.equal(some[1].cpu(), chosen[1])
+    got = gpu_ops.paged_decode_attention(q.cuda(), wide["k_cache"], wide["v_cache"], *some, k_scale=wide["k_scale"], v_scale=wide["v_scale"])
+    back = held.to(torch.int32)[chosen[0].long()]
+    check(got, *ref.decode(q, kv.k_cache, kv.v_cache, back, chosen[1], kv.k_scale, kv.v_scale), q.dtype)
+
+
 @pytest.mark.parametrize("page", [16, 32, 48, 64, 128])
 @pytest.mark.parametrize("num_splits", [0, 2])
 def test_page_sizes(gpu_ops, page, num_splits):

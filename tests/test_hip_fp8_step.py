@@ -124,3 +124,44 @@ def test_compiled_and_on_a_stream_of_its_own(gpu_ops):
     cache = dev["k"].cpu(), dev["v"].cpu()
     close(sparse, *ref.decode(q, *cache, *want, host["k_scale"], host["v_scale"]), dtype)
     close(dense, *ref.decode(q, *cache, host["block_table"], lens, host["k_scale"], host["v_scale"]), dtype)
+
+
+def test_two_captured_steps_at_once(gpu_ops):
+    """Two graphs of append, selection and both decodes, each over a cache of its own, replayed together on two streams."""
+    dtype, runs = torch.bfloat16, []
+    for i, start in enumerate(([300, 90, 17, 700], [64, 515, 1, 33])):
+        dev, host = make([n + 6 for n in start], HKV, D, PAGE)
+        g = torch.Generator().manual_seed(20 + i)
+        k, v = torch.randn(2, sum(start), HKV, D, generator=g).to(dtype)
+        off = torch.tensor([0, *start]).cumsum(0).to(torch.int32)
+        lens = torch.tensor(start, dtype=torch.int32)
+        gpu_ops.append_kv_fp8(k.cuda(), v.cuda(), dev["k"], dev["v"], dev["k_scale"], dev["v_scale"], dev["block_table"], lens.cuda(),
+                              new_offsets=off.cuda(), k_bounds=dev["bounds"])
+        ref.append(k, v, host, lens, off)
+        p = Program(gpu_ops, dev, len(start), dtype)
+        p.step()
+        torch.cuda.synchronize()
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = p.step()
+        runs.append((p, dev, host, lens, g, stream, graph, out))
+    for n in range(1, 5):
+        for p, _, _, lens, g, _, _, _ in runs:
+            p.x.copy_(torch.randn(p.x.shape, generator=g))
+            p.res.copy_(torch.randn(p.res.shape, generator=g))
+            p.lens.copy_(lens + n)
+        torch.cuda.synchronize()
+        for *_, stream, graph, _ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, dev, host, lens, _, _, _, (qkv, table, sel_lens, sparse, full) in runs:
+            qkv = qkv.cpu()
+            q = qkv[:, :HQ]
+            ref.append(qkv[:, HQ : HQ + HKV], qkv[:, HQ + HKV :], host, lens + n)
+            same(dev, host)
+            want = ref.select(q, dev["bounds"].cpu(), host["k_scale"], host["block_table"], lens + n, 4, PAGE)
+            assert torch.equal(table.cpu(), want[0]) and torch.equal(sel_lens.cpu(), want[1])
+            cache = dev["k"].cpu(), dev["v"].cpu()
+            close(sparse, *ref.decode(q, *cache, *want, host["k_scale"], host["v_scale"]), dtype)
+            close(full, *ref.decode(q, *cache, host["block_table"], lens + n, host["k_scale"], host["v_scale"]), dtype)
